@@ -312,6 +312,134 @@ VXS_API int vxs_frame_embed_device(vxs_ctx* ctx, int rows, int groups, int hidde
                                    const uint16_t* d_cp_tables, int cp_vocab, const float* d_addend,
                                    int64_t ld_addend, float* d_out, int64_t ld_out, int32_t* d_status);
 
+/*
+ * Attention over a paged cache of keys and values: the layer between the embedding of the sampled ids
+ * and the logit heads, for callers whose transformer runs on this GPU too. The reference keeps one
+ * contiguous cache per sequence (KvCache, src/Voxwerk/Talker/DecoderStack.cs:21-50) and attends with
+ * src/Voxwerk/Numerics/Attention.cs:15-118 and Rope.cs; here a layer's cache is a pool of pages that
+ * all sequences share.
+ */
+
+/* Element types of the attention entry points. */
+#define VXS_F32 0
+#define VXS_BF16 1
+#define VXS_F16 2
+
+/*
+ * One layer's cache: keys and values of `pages` pages of `page_size` tokens each. Token t of slot s
+ * (a sequence) lies in page p = table[s * ld_table + t / page_size], its key of head h at
+ *   k + p * page_stride + h * head_stride + (t % page_size) * token_stride   (elements),
+ * its value likewise in v; head_dim contiguous entries each. [pages][kv_heads][page_size][head_dim]
+ * has token_stride = head_dim, head_stride = page_size * head_dim, page_stride = kv_heads * head_stride.
+ * A host struct; k, v and table are device memory of the caller's, which also owns the choice of
+ * pages (several slots may hold the same page). page_size is a power of two from 16 to 65536, head_dim
+ * 64, 128 or 256, the strides are multiples of 8, k and v 16-byte aligned (else VXS_ERR_UNSUPPORTED).
+ */
+typedef struct vxs_kv_cache {
+    void* k;
+    void* v;
+    const int32_t* table; /* [slots][ld_table] page numbers; entries past a sequence's end are not used */
+    int64_t ld_table;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t token_stride;
+    int32_t slots;
+    int32_t pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t dtype; /* VXS_BF16 or VXS_F16 */
+} vxs_kv_cache;
+
+/*
+ * What happens to a query or key head before attention: an RMS norm over its entries (weights fp32
+ * [head_dim] in device memory; NULL: none), then the rotation of its first rot_dim entries in pairs:
+ * entries i and i + rot_dim / 2 (interleaved 0) or 2i and 2i + 1 (interleaved 1) turn by
+ * position * inv_freq[i] radians, inv_freq fp32 [rot_dim / 2] in device memory (rot_dim 0: no
+ * rotation). rope_scale multiplies both cosine and sine (1, or the magnitude that a scaling for
+ * long contexts asks for). rot_dim is a multiple of 8.
+ */
+typedef struct vxs_kv_prep {
+    const float* q_norm;
+    const float* k_norm;
+    const float* inv_freq;
+    float eps;
+    float rope_scale;
+    int32_t rot_dim;
+    int32_t interleaved;
+} vxs_kv_prep;
+
+/*
+ * The projections of `tokens` new tokens on their way to attention, in one pass: each query and key head
+ * is normed and rotated (prep; NULL: neither), queries go to q_out, keys and values to their pages.
+ *   q, k, v    [tokens] rows of q_heads, kv_heads and kv_heads heads of head_dim entries, of in_dtype, with
+ *              leading dimensions ldq, ldk, ldv in elements (a packed projection passes three places of one
+ *              buffer); q or k and v may be NULL: only the others are done
+ *   d_pos      int32 [tokens] positions of the rotation; may be NULL where nothing rotates and d_index is given
+ *   d_slots    int32 [tokens] each token's slot; NULL: token t belongs to slot t (one new token per sequence)
+ *   d_index    int32 [tokens] each token's place in its sequence; NULL: d_pos
+ *   q_out      [tokens] rows of the cache's dtype, leading dimension ldqo
+ *   d_status   NULL or int32 [tokens]: 0, or VXS_ERR_ID_OUT_OF_RANGE for a token whose slot, place or page lies
+ *              outside the cache: its key and value are not written
+ * Norms, angles and products are fp32 or wider, rounded once, to nearest even. Pointers 16-byte (fp32) or 8-byte
+ * (bf16, fp16) aligned, leading dimensions multiples of 4 (q_out: 8-byte, 4), else VXS_ERR_UNSUPPORTED. Two tokens
+ * of one call with the same place leave either. Asynchronous on the context stream.
+ */
+VXS_API int vxs_kv_append_device(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, const void* k,
+                                 int64_t ldk, const void* v, int64_t ldv, int in_dtype, const vxs_kv_prep* prep,
+                                 const int32_t* d_pos, const int32_t* d_slots, const int32_t* d_index,
+                                 const vxs_kv_cache* cache, void* q_out, int64_t ldqo, int32_t* d_status);
+
+/*
+ * Causal attention of packed sequences over their pages: sequence i (slot d_slots[i]; NULL: slot i) has new tokens
+ * [d_q_off[i], d_q_off[i + 1]) of the `tokens` query rows and d_kv_len[i] tokens in the cache, the new ones last
+ * (appended before): its j-th of n new tokens sees the keys up to and with d_kv_len[i] - n + j. For each query head
+ * h (key head h / (q_heads / kv_heads)):
+ *   out[t][h] = sum_s softmax_s(scale * q[t][h] . k[s]) v[s]
+ * A token that sees no key gets zeros; keys that a token does not see do not touch its result, whatever they hold.
+ * q is of the cache's dtype, out of that or VXS_F32 (leading dimensions in elements, multiples of 8, 16-byte
+ * aligned, else VXS_ERR_UNSUPPORTED); scale is positive and finite, q_heads a multiple of kv_heads. Sums and softmax
+ * statistics are fp32; the weights are rounded to the cache's type for the matrix cores, and for fp32 outputs kept
+ * to twice its bits. Rows outside every sequence are not written; a slot outside the cache has no keys, a length above
+ * the table's is cut to it. Asynchronous on the context stream.
+ */
+VXS_API int vxs_attn_prompt_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,
+                                   const vxs_kv_cache* cache, const int32_t* d_slots, const int32_t* d_q_off,
+                                   const int32_t* d_kv_len, float scale, void* out, int64_t ldo, int out_dtype);
+
+/*
+ * A prefix that groups of rows share (the same voice or instructions): rows [d_off[g], d_off[g + 1]) hold the same
+ * pages, or copies of the same entries, for their first d_len[g] tokens, which are read once for all of them, from the
+ * first row's pages. d_off int32 [groups + 1] (ascending) and d_len int32 [groups] in device memory; max_len: no
+ * d_len is longer. Rows outside every group share nothing.
+ */
+typedef struct vxs_shared_prefix {
+    const int32_t* d_off;
+    const int32_t* d_len;
+    int32_t groups;
+    int32_t max_len;
+} vxs_shared_prefix;
+
+/*
+ * Attention of one token per sequence: row r's query heads over the first d_kv_len[r] tokens of its slot
+ * (d_slots[r]; NULL: slot r), its own among them. Results, types and layouts as vxs_attn_prompt_device; a row of
+ * length 0 gets zeros. max_len: no length is longer (the work is divided for it; a longer one costs time, not
+ * correctness). prefix: NULL, or the rows' shared prefixes.
+ *
+ * work: device memory of vxs_attn_step_workspace bytes, 16-byte aligned, zeroed once before its first use; calls
+ * leave it ready for the next. One call at a time may use it (calls on one stream are in order). NULL: each row's keys
+ * are read by one workgroup per key head, with no sharing.
+ * Asynchronous on the context stream; may be captured.
+ */
+VXS_API int vxs_attn_step_device(vxs_ctx* ctx, int rows, int q_heads, const void* q, int64_t ldq,
+                                 const vxs_kv_cache* cache, const int32_t* d_slots, const int32_t* d_kv_len, int max_len,
+                                 const vxs_shared_prefix* prefix, float scale, void* out, int64_t ldo, int out_dtype,
+                                 void* work, int64_t work_bytes);
+
+/* The workspace of vxs_attn_step_device calls of at most these sizes, in bytes; negative: an error code. */
+VXS_API int64_t vxs_attn_step_workspace(vxs_ctx* ctx, int rows, int q_heads, const vxs_kv_cache* cache, int max_len,
+                                        const vxs_shared_prefix* prefix);
+
 #ifdef __cplusplus
 }
 #endif

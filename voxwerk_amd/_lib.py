@@ -31,6 +31,7 @@ VXS_FLAG_PATH_BLOCK = 1 << 8
 VXS_FLAG_PATH_WAVE = 1 << 9
 VXS_FLAG_RNG_TALKER = 1 << 10
 VXS_FLAG_RNG_SUB = 1 << 11
+VXS_F32, VXS_BF16, VXS_F16 = 0, 1, 2
 
 
 class VxsParams(ctypes.Structure):
@@ -79,6 +80,27 @@ class VxsWorkload(ctypes.Structure):
     ]
 
 
+class VxsKvCache(ctypes.Structure):
+    """vxs_kv_cache (include/vxs_sampler.h)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("ld_table", c_int64), ("page_stride", c_int64),
+                ("head_stride", c_int64), ("token_stride", c_int64), ("slots", c_int32), ("pages", c_int32),
+                ("page_size", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32)]
+
+
+class VxsKvPrep(ctypes.Structure):
+    """vxs_kv_prep (include/vxs_sampler.h)."""
+
+    _fields_ = [("q_norm", c_void_p), ("k_norm", c_void_p), ("inv_freq", c_void_p), ("eps", c_float),
+                ("rope_scale", c_float), ("rot_dim", c_int32), ("interleaved", c_int32)]
+
+
+class VxsSharedPrefix(ctypes.Structure):
+    """vxs_shared_prefix (include/vxs_sampler.h)."""
+
+    _fields_ = [("d_off", c_void_p), ("d_len", c_void_p), ("groups", c_int32), ("max_len", c_int32)]
+
+
 _P = c_void_p  # raw pointers are passed as integers / c_void_p
 
 _SIGNATURES = {
@@ -108,6 +130,13 @@ _SIGNATURES = {
     "vxs_head_pack_int8_device": (c_int, [c_void_p, c_int, c_int, _P, c_int64, _P, c_int64, _P]),
     "vxs_frame_embed_device": (c_int, [c_void_p, c_int, c_int, c_int, _P, c_int64, c_int64, _P, c_int, _P, c_int, _P,
                                        c_int64, _P, c_int64, _P]),
+    "vxs_kv_append_device": (c_int, [c_void_p, c_int, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P, _P, _P,
+                                     _P, _P, c_int64, _P]),
+    "vxs_attn_prompt_device": (c_int, [c_void_p, c_int, c_int, c_int, _P, c_int64, _P, _P, _P, _P, c_float, _P, c_int64,
+                                       c_int]),
+    "vxs_attn_step_device": (c_int, [c_void_p, c_int, c_int, _P, c_int64, _P, _P, _P, c_int, _P, c_float, _P, c_int64,
+                                     c_int, _P, c_int64]),
+    "vxs_attn_step_workspace": (c_int64, [c_void_p, c_int, c_int, _P, c_int, _P]),
     "vxs_history_draw": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, _P]),
     "vxs_sample_batch": (c_int, [c_void_p, c_void_p, c_int, c_int, _P, c_int64, _P, c_int, _P, c_int, _P, _P,
                                  c_uint32]),

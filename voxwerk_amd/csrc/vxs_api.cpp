@@ -590,6 +590,18 @@ int fetch_ok_rows(vxs_ctx* ctx, void* dst, const void* src, const int32_t* ids, 
 
 }  // namespace
 
+namespace vxs {
+
+int ctx_fail(vxs_ctx* ctx, int code, const char* msg) { return fail(ctx, code, msg); }
+int ctx_hip_fail(vxs_ctx* ctx, hipError_t e, const char* what) { return hip_fail(ctx, e, what); }
+hipError_t ctx_use(vxs_ctx* ctx) { return hipSetDevice(ctx->device); }
+int ctx_ok(vxs_ctx* ctx) {
+    ctx->err.clear();
+    return VXS_OK;
+}
+
+}  // namespace vxs
+
 extern "C" {
 
 VXS_API const char* vxs_version(void) { return "vxs 0.1.0 gfx950"; }

@@ -289,4 +289,10 @@ bool split_wanted(const SampleArgs& a);
 // n successive NextDouble() of one generator into out[0..n) (one thread; a check and debug aid).
 hipError_t launch_draw_sequence(int32_t* state, int n, double* out, hipStream_t stream);
 
+// A context for entry points outside vxs_api.cpp: its error text and code, its device made current, success.
+int ctx_fail(vxs_ctx* ctx, int code, const char* msg);
+int ctx_hip_fail(vxs_ctx* ctx, hipError_t e, const char* what);
+hipError_t ctx_use(vxs_ctx* ctx);
+int ctx_ok(vxs_ctx* ctx);
+
 }  // namespace vxs

@@ -17,6 +17,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import PARAMS_DTYPE, load_vxs, ptr
+from .attention import DTYPES, KvCache, KvPrep, SharedPrefix
 
 
 class SamplerError(RuntimeError):
@@ -405,6 +406,40 @@ class Context:
         self._check(self._lib.vxs_frame_embed_device(self._h, rows, groups, hidden, ptr(codes), ld_codes, group_stride,
                                                      ptr(codec_table), vocab, ptr(cp_tables), cp_vocab, ptr(addend),
                                                      ld_addend, ptr(out), ld_out, ptr(status)))
+
+    # attention over a paged cache (device pointers, asynchronous; voxwerk_amd.attention has the structures) ----
+    def kv_append_device(self, tokens: int, q_heads: int, q, ldq: int, k, ldk: int, v, ldv: int, in_dtype: str,
+                         cache: KvCache, pos, slots, q_out, ld_q_out: int, prep: Optional[KvPrep] = None, index=None,
+                         status=None) -> None:
+        """vxs_kv_append_device: norm and rotate new tokens' query and key heads, queries to q_out, keys and values
+        to their pages."""
+        self._check(self._lib.vxs_kv_append_device(
+            self._h, tokens, q_heads, ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, DTYPES[in_dtype],
+            prep.ref if prep is not None else None, ptr(pos), ptr(slots), ptr(index), cache.ref, ptr(q_out), ld_q_out,
+            ptr(status)))
+
+    def attn_prompt_device(self, seqs: int, tokens: int, q_heads: int, q, ldq: int, cache: KvCache, q_off, kv_len,
+                           scale: float, out, ldo: int, out_dtype: str, slots=None) -> None:
+        """vxs_attn_prompt_device: causal attention of packed sequences' new tokens over their pages."""
+        self._check(self._lib.vxs_attn_prompt_device(self._h, seqs, tokens, q_heads, ptr(q), ldq, cache.ref, ptr(slots),
+                                                     ptr(q_off), ptr(kv_len), scale, ptr(out), ldo, DTYPES[out_dtype]))
+
+    def attn_step_workspace(self, rows: int, q_heads: int, cache: KvCache, max_len: int,
+                            prefix: Optional[SharedPrefix] = None) -> int:
+        """vxs_attn_step_workspace: the bytes of zeroed device memory that steps of these sizes work in."""
+        n = self._lib.vxs_attn_step_workspace(self._h, rows, q_heads, cache.ref, max_len,
+                                              prefix.ref if prefix is not None else None)
+        self._check(min(n, 0))
+        return n
+
+    def attn_step_device(self, rows: int, q_heads: int, q, ldq: int, cache: KvCache, kv_len, max_len: int, scale: float,
+                         out, ldo: int, out_dtype: str, slots=None, prefix: Optional[SharedPrefix] = None,
+                         workspace=None, workspace_bytes: int = 0) -> None:
+        """vxs_attn_step_device: attention of one token per sequence over its pages, shared prefixes read once."""
+        self._check(self._lib.vxs_attn_step_device(
+            self._h, rows, q_heads, ptr(q), ldq, cache.ref, ptr(slots), ptr(kv_len), max_len,
+            prefix.ref if prefix is not None else None, scale, ptr(out), ldo, DTYPES[out_dtype], ptr(workspace),
+            workspace_bytes))
 
 
 class HistoryStore:
