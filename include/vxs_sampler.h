@@ -333,7 +333,7 @@ VXS_API int vxs_frame_embed_device(vxs_ctx* ctx, int rows, int groups, int hidde
  * has token_stride = head_dim, head_stride = page_size * head_dim, page_stride = kv_heads * head_stride.
  * A host struct; k, v and table are device memory of the caller's, which also owns the choice of
  * pages (several slots may hold the same page). page_size is a power of two from 16 to 65536, head_dim
- * 64, 128 or 256, the strides are multiples of 8, k and v 16-byte aligned (else VXS_ERR_UNSUPPORTED).
+ * 64, 128 or 256, the strides are multiples of 8 (token_stride below 2^25, page_stride below 2^31), k and v 16-byte aligned (else VXS_ERR_UNSUPPORTED).
  */
 typedef struct vxs_kv_cache {
     void* k;

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a) {
     const int qh = a.q ? a.q_heads : 0, kh = a.k ? a.cache.kv_heads : 0;
     const int heads = qh + 2 * kh;
     // this lane's two runs
-    const bool turned = inter ? 8 * u < rot : 8 * u < rot;
+    const bool turned = 8 * u < rot;
     const int ra = inter ? 8 * u : turned ? 4 * u : rot + (4 * u - rot / 2);
     const int rb = inter ? 8 * u + 4 : ra + (turned ? rot / 2 : (D - rot) / 2);
     f4 c{1.f, 1.f, 1.f, 1.f}, s{0.f, 0.f, 0.f, 0.f};
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a) {
         if ((unsigned)slot < (unsigned)a.cache.slots && place >= 0 && (place >> a.cache.page_bits) < a.cache.ld_table) {
             const int page = a.cache.table[(int64_t)slot * a.cache.ld_table + (place >> a.cache.page_bits)];
             if ((unsigned)page < (unsigned)a.cache.pages)
-                at = (int64_t)page * a.cache.page_stride + (int64_t)(place & ((1 << a.cache.page_bits) - 1)) * a.cache.token_stride;
+                at = (int64_t)cache_offset(a.cache, page, 0, place);
         }
     }
     if (a.status && threadIdx.x == 0 && blockIdx.y == 0) a.status[t] = kh && at < 0 ? VXS_ERR_ID_OUT_OF_RANGE : 0;

@@ -14,7 +14,8 @@ struct PagedCache {
     char* v;
     const int32_t* table;
     int64_t ld_table;
-    int64_t page_stride, head_stride, token_stride;  // bytes
+    int64_t head_stride;                 // bytes
+    uint32_t page_stride, token_stride;  // bytes
     int slots, pages, page_bits, kv_heads, head_dim;
 };
 
@@ -64,11 +65,11 @@ __device__ __forceinline__ int64_t cache_length(const PagedCache& c, int slot, i
     return len < most ? len : most;
 }
 
-// Byte offset, from k or v, of token t's entries of head h; t < cache_length. A page number outside the pool
-// (a caller's mistake) reads some page of it.
-__device__ __forceinline__ int64_t cache_offset(const PagedCache& c, const int32_t* pages_of_slot, int h, int t) {
-    const unsigned p = min((unsigned)pages_of_slot[t >> c.page_bits], (unsigned)c.pages - 1u);
-    return (int64_t)p * c.page_stride + (int64_t)h * c.head_stride + (int64_t)(t & ((1 << c.page_bits) - 1)) * c.token_stride;
+// Byte offset, from k or v, of token t's entries of head h, whose table entry is `page`. A page number outside the
+// pool (a caller's mistake) reads some page of it.
+__device__ __forceinline__ uint64_t cache_offset(const PagedCache& c, int page, int h, int t) {
+    return (uint64_t)min((unsigned)page, (unsigned)c.pages - 1u) * c.page_stride + (uint64_t)h * c.head_stride +
+           (uint64_t)((unsigned)t & ((1u << c.page_bits) - 1u)) * c.token_stride;
 }
 #endif
 

@@ -38,13 +38,15 @@ int check_cache(vxs_ctx* ctx, const vxs_kv_cache* c, int q_heads, vxs::PagedCach
     // Token numbers are 32-bit in the kernels (tiles may run up to 256 past the end).
     if (c->ld_table > (INT32_MAX - 256) / c->page_size)
         return ctx_fail(ctx, VXS_ERR_UNSUPPORTED, "ld_table * page_size must stay below 2^31 - 256");
+    if (c->token_stride > INT32_MAX / 64 || c->page_stride > INT32_MAX || c->head_stride > INT64_MAX / 65536)
+        return ctx_fail(ctx, VXS_ERR_UNSUPPORTED, "token_stride must stay below 2^25, page_stride below 2^31");
     out.k = static_cast<char*>(c->k);
     out.v = static_cast<char*>(c->v);
     out.table = c->table;
     out.ld_table = c->ld_table;
-    out.page_stride = 2 * c->page_stride;
+    out.page_stride = (uint32_t)(2 * c->page_stride);
     out.head_stride = 2 * c->head_stride;
-    out.token_stride = 2 * c->token_stride;
+    out.token_stride = (uint32_t)(2 * c->token_stride);
     out.slots = c->slots;
     out.pages = c->pages;
     out.page_bits = __builtin_ctz((unsigned)c->page_size);

@@ -1,0 +1,307 @@
+// vxs_attn_core.h — what the attention kernels share: tiles of a paged cache on their way into LDS, and a wave's
+// products with them on the matrix cores.
+//
+// A wave holds 32 query rows as the columns of 32x32x16 products. Scores come transposed, S^T = K Q^T: lane l has
+// column c = l % 32 and, of each 32 keys, those 8 j + 4 (l / 32) + 0..3, j = 0..3, in 16 registers. So a query's
+// maximum and sum stay within two lanes, rescaling is one factor per lane, and the weights are the second product's
+// right operand where they are: O^T = V^T P^T, whose sum over keys may take them in any order as long as V^T's
+// operand has the same one. V^T comes from the row-major tile through the transposing LDS read (16 lanes give four
+// rows of 16 entries and get four keys of one entry each).
+//
+// A tile in LDS has its rows' 16-byte units at their index xor swizzle(row): the 16 rows at one unit that a K read
+// touches at a time, and the 4 rows at 4 units of a V read, then lie in different banks. Tiles are loaded straight into
+// LDS, 1 KiB a wave instruction in lane order; the swizzle is in the addresses that the lanes load from, whose rows
+// stay whole.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "vxs_attn.h"
+
+namespace vxs {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<__bf16> {
+    using v4 = bf4;
+    using v8 = bf8;
+    static constexpr unsigned kExponent = 0x7F80u;  // all ones: infinity or NaN
+    static __device__ __forceinline__ f16v mfma(bf8 a, bf8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Vec<_Float16> {
+    using v4 = h4;
+    using v8 = h8;
+    static constexpr unsigned kExponent = 0x7C00u;
+    static __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Vec<float> {
+    using v4 = f4;
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {  // (a NaN loses, as in fmaxf, with nothing to canonicalise)
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+// The larger of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.0e38f;  // a running maximum before any key
+// Weights are exp2(score - m) for an m that may lag behind the maximum by this much: the sums are rescaled only when
+// some query's maximum has grown by more, and no weight passes 2^8.
+constexpr float kLag = 8.0f;
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {  // all but the N youngest loads into LDS have arrived
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+template <int D>
+struct TileGeom {
+    static constexpr int kRow = 2 * D;           // bytes
+    static constexpr int kUnits = D / 8;         // 16-byte units of a row
+    static constexpr int kRows = 64 / kUnits;    // rows of one load instruction
+    static constexpr int kLoads = 16 / kRows;    // of 16 rows
+    static __device__ __forceinline__ int swizzle(int row) {
+        return D >= 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    }
+};
+
+// Loads of 16 rows (a granule: always within one page) of a cache into LDS.
+template <int D>
+struct Loader {
+    using G = TileGeom<D>;
+    unsigned off[G::kLoads];  // this lane's byte offsets within a granule
+    __device__ __forceinline__ void init(const PagedCache& c, int lane) {
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++) {
+            const int row = j * G::kRows + lane / G::kUnits;
+            off[j] = (unsigned)row * (unsigned)c.token_stride + 16u * (unsigned)((lane % G::kUnits) ^ G::swizzle(row));
+        }
+    }
+    // base: the granule's first row (uniform); lds: where its rows go
+    __device__ __forceinline__ void load(const char* base, unsigned lds) const {
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + 1024u * j), "v"(off[j]), "s"(base)
+                         : "memory");
+    }
+};
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const char* uniform_ptr(const char* p) {
+    const uint64_t x = (uint64_t)p;
+    return (const char*)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
+}
+
+// Read-only memory of the launch, read with scalar loads: they are not counted with the loads into LDS.
+template <typename A>
+using Constant = const __attribute__((address_space(4))) A;
+__device__ __forceinline__ int scalar(const int32_t* p, int64_t i) { return ((Constant<int32_t>*)p)[i]; }
+// The kernel's arguments (of type A, the first) read again: kept from the start they would hold registers throughout.
+template <typename A>
+__device__ __forceinline__ A arguments_again() {
+#ifdef __HIP_DEVICE_COMPILE__
+    Constant<A>* p = (Constant<A>*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+#else
+    return A{};
+#endif
+}
+
+// Byte offset, from k or v at `head`, of the granule that begins at token t (uniform) of a slot whose table entries are
+// `pages`, the last of them that is used at `last`. Granules past the end read what is there in the pool.
+__device__ __forceinline__ uint64_t granule_offset(const PagedCache& c, const int32_t* pages, int last, int t) {
+    return cache_offset(c, scalar(pages, min(t >> c.page_bits, last)), 0, t);
+}
+
+// A wave's 32 queries: operand, running maximum, sum of its own keys' weights, and outputs O^T.
+template <int D, typename T, bool SPLIT>
+struct Queries {
+    using G = TileGeom<D>;
+    using v8 = typename Vec<T>::v8;
+    v8 q[D / 16];
+    f16v o[D / 32];
+    float m, l;
+
+    __device__ __forceinline__ void init() {
+        m = kLowest;
+        l = 0.f;
+#pragma unroll
+        for (int b = 0; b < D / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[b][i] = 0.f;
+    }
+    // row: this lane's query (null: zeros); the 8 entries at 16 t + 8 (lane / 32) are the lane's for step t
+    __device__ __forceinline__ void load(const T* row, int lane) {
+#pragma unroll
+        for (int t = 0; t < D / 16; t++) {
+            v8 x{};
+            if (row) x = *reinterpret_cast<const v8*>(row + 16 * t + 8 * (lane >> 5));
+            q[t] = x;
+        }
+    }
+    __device__ __forceinline__ void loaded() {  // the wait for load() is here (and for every load into LDS before)
+#pragma unroll
+        for (int t = 0; t < D / 16; t++) asm volatile("" : "+v"(q[t]));
+    }
+
+    // S^T of 32 keys at `tile`
+    __device__ __forceinline__ f16v scores(const char* tile, int lane) const {
+        const int row = lane & 31;
+        const char* p = tile + row * G::kRow;
+        const int u = ((lane >> 5) ^ G::swizzle(row)) << 4;
+        f16v s{};
+#pragma unroll
+        for (int t = 0; t < D / 16; t++) s = Vec<T>::mfma(*reinterpret_cast<const v8*>(p + ((32 * t) ^ u)), q[t], s);
+        return s;
+    }
+
+    // Weights of NB x 32 keys from their scores; c = scale log2 e. The sums are rescaled when they have to be.
+    template <int NB>
+    __device__ __forceinline__ void weigh(f16v (&s)[NB], float c) {
+        float top = kLowest;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) top = max3(top, s[b][i], s[b][i + 1]);
+        top = max_halves(top) * c;
+        if (__ballot(top > m + kLag)) {
+            const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= shrink;
+#pragma unroll
+            for (int b = 0; b < D / 32; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] *= shrink;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, -m));
+                part[i & 3] += s[b][i];
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
+        }
+    }
+
+    // Unseen keys of a tile have no weight: this lane's query sees `seen` of its keys (which may be negative or more).
+    template <int NB>
+    static __device__ __forceinline__ void hide(f16v (&s)[NB], int seen, int lane) {
+        seen -= 4 * (lane >> 5);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (32 * b + 8 * (i >> 2) + (i & 3) >= seen) s[b][i] = -__builtin_inff();
+    }
+
+    // Four keys of 32 entries of V^T, twice: rows 16 t + 8 u + 4 (lane / 32) + 0..3 of `tile`, entries 32 b + lane % 32.
+    static __device__ __forceinline__ s8 values(const char* tile, int t, int b, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        const int row = 4 * (g >> 1) + (i >> 2);
+        const int unit = (2 * (g & 1) + ((i & 3) >> 1)) ^ G::swizzle(row);
+        const char* p = tile + row * G::kRow + 8 * (i & 1);
+        using lds_s4 = __attribute__((address_space(3))) s4;
+        // (8 rows further the swizzle differs in bit 1)
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 16 * t * G::kRow + ((64 * b) ^ (unit << 4))));
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * t + 8) * G::kRow + ((64 * b) ^ (unit << 4) ^ 32)));
+        return s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    }
+    static __device__ __forceinline__ v8 weights(const f16v& s, int t, v8& rest) {
+        v8 hi;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            hi[e] = (T)s[8 * t + e];
+            if (SPLIT) rest[e] = (T)(s[8 * t + e] - (float)hi[e]);
+        }
+        return hi;
+    }
+
+    enum Mask {
+        kAll,   // every query sees every key of the tile
+        kTail,  // all queries see the same first `seen` keys: the others' values are taken as zero
+        kEach,  // each query sees its own first `seen` keys
+    };
+
+    // O^T += V^T P^T over NB x 32 keys. The weights are rounded to T once (SPLIT: the rest of each in a second product).
+    // A weight of zero does not hide an infinite or NaN value from the sum, so with kTail values past the end are
+    // zeroed, and with kEach values that are not finite are zeroed, then added for the queries that see them.
+    template <int NB, Mask MASK>
+    __device__ __forceinline__ void add(const char* tile, const f16v (&s)[NB], int seen, int lane) {
+        // (the rarer forms form their addresses anew: kept from tile to tile they would cost registers)
+        if (MASK != kAll) asm volatile("" : "+v"(lane));
+        v8 hi[2 * NB], lo[2 * NB];
+#pragma unroll
+        for (int k = 0; k < 2 * NB; k++) hi[k] = weights(s[k >> 1], k & 1, lo[k]);
+        unsigned odd = 0;
+#pragma unroll
+        for (int b = 0; b < D / 32; b++)
+#pragma unroll
+            for (int k = 0; k < 2 * NB; k++) {
+                s8 v = values(tile, k, b, lane);
+                if (MASK == kTail) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (16 * k + 8 * (e >> 2) + (e & 3) >= seen - 4 * (lane >> 5)) v[e] = 0;
+                }
+                if (MASK == kEach) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (((unsigned short)v[e] & Vec<T>::kExponent) == Vec<T>::kExponent) {
+                            v[e] = 0;
+                            odd = 1;
+                        }
+                }
+                const v8 a = __builtin_bit_cast(v8, v);
+                o[b] = Vec<T>::mfma(a, hi[k], o[b]);
+                if (SPLIT) o[b] = Vec<T>::mfma(a, lo[k], o[b]);
+            }
+        if (MASK == kEach && __ballot(odd != 0)) {
+            for (int key = 0; key < 32 * NB; key++) {
+                const char* row = tile + key * G::kRow + 8 * (lane >> 5);
+                const int sw = G::swizzle(key) << 4;
+#pragma unroll
+                for (int b = 0; b < D / 32; b++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const s4 x = *reinterpret_cast<const s4*>(row + ((64 * b + 16 * j) ^ sw));
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (((unsigned short)x[e] & Vec<T>::kExponent) == Vec<T>::kExponent && key < seen)
+                                o[b][4 * j + e] += (float)__builtin_bit_cast(T, (short)x[e]);
+                        asm volatile("" ::: "memory");  // (one read at a time: this may be slow, not large)
+                    }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void finish_sum() { l += __shfl_xor(l, 32); }
+};
+
+}  // namespace vxs

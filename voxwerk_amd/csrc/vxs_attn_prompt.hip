@@ -1,13 +1,12 @@
-// vxs_attn.hip — attention over a paged cache: packed prompts, and one token per sequence.
+// vxs_attn.hip — attention of packed prompts over a paged cache.
 //
 //   out[r] = sum_s w_s v[s] / sum_s w_s,   w_s = exp(scale q[r] . k[s] - m)   over the keys s that row r sees,
 // with the running maximum m and both sums carried along the keys (when m grows by d, the sums shrink by exp(-d)).
 // Here one wave per query row and head goes over its keys one after the other, each lane holding D/64 entries.
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "vxs_attn.h"
+#include "vxs_attn_types.h"
 
 namespace vxs {
 namespace {
@@ -24,7 +23,7 @@ __device__ __forceinline__ void attend_row(const PagedCache& c, const T* q, int 
     float m = -3.0e38f, l = 0.f;
     const int32_t* pages = c.table + (int64_t)slot * c.ld_table;
     for (int t = 0; t < n; t++) {
-        const int64_t at = cache_offset(c, pages, h, t);
+        const uint64_t at = cache_offset(c, pages[t >> c.page_bits], h, t);
         const T* k = reinterpret_cast<const T*>(c.k + at) + lane * E;
         const T* v = reinterpret_cast<const T*>(c.v + at) + lane * E;
         float s = 0.f;
@@ -57,53 +56,16 @@ __global__ __launch_bounds__(64) void prompt_kernel(PromptArgs a) {
 }
 
 template <int D, typename T, typename TO>
-__global__ __launch_bounds__(64) void step_kernel(StepArgs a) {
-    const int r = blockIdx.x, head = blockIdx.y;
-    const int slot = a.slots ? a.slots[r] : r;
-    const int64_t n = cache_length(a.cache, slot, a.kv_len[r]);
-    attend_row<D>(a.cache, static_cast<const T*>(a.q) + r * a.ldq + (int64_t)head * D, n > 0 ? slot : 0,
-                  head / (a.q_heads / a.cache.kv_heads), n, a.scale, static_cast<TO*>(a.out) + r * a.ldo + (int64_t)head * D);
-}
-
-template <template <int, typename, typename> class F, typename A>
-hipError_t by_type(const A& a, int dtype, int out_dtype, hipStream_t stream) {
-    auto dim = [&](auto d) {
-        constexpr int D = decltype(d)::value;
-        if (dtype == VXS_BF16) return out_dtype == VXS_F32 ? F<D, __bf16, float>::go(a, stream) : F<D, __bf16, __bf16>::go(a, stream);
-        return out_dtype == VXS_F32 ? F<D, _Float16, float>::go(a, stream) : F<D, _Float16, _Float16>::go(a, stream);
-    };
-    switch (a.cache.head_dim) {
-        case 64: return dim(std::integral_constant<int, 64>{});
-        case 128: return dim(std::integral_constant<int, 128>{});
-        default: return dim(std::integral_constant<int, 256>{});
-    }
-}
-
-template <int D, typename T, typename TO>
 struct Prompt {
     static hipError_t go(const PromptArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL((prompt_kernel<D, T, TO>), dim3(a.tokens, a.q_heads), dim3(64), 0, stream, a);
         return hipGetLastError();
     }
 };
-template <int D, typename T, typename TO>
-struct Step {
-    static hipError_t go(const StepArgs& a, hipStream_t stream) {
-        hipLaunchKernelGGL((step_kernel<D, T, TO>), dim3(a.rows, a.q_heads), dim3(64), 0, stream, a);
-        return hipGetLastError();
-    }
-};
-
 }  // namespace
 
 hipError_t launch_attn_prompt(const PromptArgs& a, int dtype, int out_dtype, hipStream_t stream) {
-    return by_type<Prompt>(a, dtype, out_dtype, stream);
-}
-
-int64_t attn_step_work_bytes(const StepArgs&) { return 0; }
-
-hipError_t launch_attn_step(const StepArgs& a, int dtype, int out_dtype, hipStream_t stream) {
-    return by_type<Step>(a, dtype, out_dtype, stream);
+    return by_type<Prompt>(a, a.cache.head_dim, dtype, out_dtype, stream);
 }
 
 }  // namespace vxs
