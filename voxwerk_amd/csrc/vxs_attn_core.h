@@ -38,6 +38,7 @@ struct Vec<__bf16> {
     using v4 = bf4;
     using v8 = bf8;
     static constexpr unsigned kExponent = 0x7F80u;  // all ones: infinity or NaN
+    static constexpr float kAbove = 8.0f;           // = kLag: m over the maximum when it is set
     static __device__ __forceinline__ f16v mfma(bf8 a, bf8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -45,6 +46,7 @@ struct Vec<_Float16> {
     using v4 = h4;
     using v8 = h8;
     static constexpr unsigned kExponent = 0x7C00u;
+    static constexpr float kAbove = 0.0f;
     static __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -65,8 +67,10 @@ __device__ __forceinline__ float max_halves(float x) {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.0e38f;  // a running maximum before any key
-// Weights are exp2(score - m) for an m that may lag behind the maximum by this much: the sums are rescaled only when
-// some query's maximum has grown by more, and no weight passes 2^8.
+// Weights are exp2(score - m), and the sums are rescaled only when some query's maximum has grown by more than kLag since
+// m was set: to the maximum for fp16, whose weights then lie where its precision is and reach 2^kLag (its values end
+// at 2^16, so no sum overflows); for bf16 to kLag above it, so that no weight passes 1 and the type's largest values can be
+// averaged.
 constexpr float kLag = 8.0f;
 
 template <int N>
@@ -189,8 +193,8 @@ struct Queries {
 #pragma unroll
             for (int i = 0; i < 16; i += 2) top = max3(top, s[b][i], s[b][i + 1]);
         top = max_halves(top) * c;
-        if (__ballot(top > m + kLag)) {
-            const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - next);
+        if (__ballot(top > m + (kLag - Vec<T>::kAbove))) {
+            const float next = fmaxf(m, top + Vec<T>::kAbove), shrink = __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= shrink;
 #pragma unroll

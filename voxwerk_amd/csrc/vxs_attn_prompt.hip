@@ -1,67 +1,124 @@
-// vxs_attn.hip — attention of packed prompts over a paged cache.
+// vxs_attn_prompt.hip — causal attention of packed sequences' new tokens over a paged cache.
 //
-//   out[r] = sum_s w_s v[s] / sum_s w_s,   w_s = exp(scale q[r] . k[s] - m)   over the keys s that row r sees,
-// with the running maximum m and both sums carried along the keys (when m grows by d, the sums shrink by exp(-d)).
-// Here one wave per query row and head goes over its keys one after the other, each lane holding D/64 entries.
+// Token j of a sequence's n new ones (of `len` in the cache) sees its keys s < len - n + j + 1:
+//   out[t] = sum_s w_s v[s] / sum_s w_s,   w_s = exp(scale q[t] . k[s] - m)
+// carried along the keys with the running maximum m.
+//
+// Bound by the matrix cores: 4 D operations for each query head and key that it sees. The query heads of one key head
+// are stacked, row rho = j G + g for token j and head g of G, so all rows of a workgroup read the same keys: a wave
+// holds 32 rows (vxs_attn_core.h), the four waves of a workgroup 128 consecutive ones, and each tile of 64 keys is loaded
+// into LDS once for all four, the next one while this one is used.
 #include <hip/hip_runtime.h>
 
-#include "vxs_attn.h"
+#include <algorithm>
+
+#include "vxs_attn_core.h"
 #include "vxs_attn_types.h"
 
 namespace vxs {
 namespace {
 
-template <int D, typename T, typename TO>
-__device__ __forceinline__ void attend_row(const PagedCache& c, const T* q, int slot, int h, int64_t n, float scale, TO* out) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    float x[E], acc[E];
-    for (int e = 0; e < E; e++) {
-        x[e] = (float)q[lane * E + e] * scale;
-        acc[e] = 0.f;
-    }
-    float m = -3.0e38f, l = 0.f;
-    const int32_t* pages = c.table + (int64_t)slot * c.ld_table;
-    for (int t = 0; t < n; t++) {
-        const uint64_t at = cache_offset(c, pages[t >> c.page_bits], h, t);
-        const T* k = reinterpret_cast<const T*>(c.k + at) + lane * E;
-        const T* v = reinterpret_cast<const T*>(c.v + at) + lane * E;
-        float s = 0.f;
-        for (int e = 0; e < E; e++) s = __builtin_fmaf(x[e], (float)k[e], s);
-        for (int b = 32; b >= 1; b /= 2) s += __shfl_xor(s, b);
-        const float top = fmaxf(m, s), old = __expf(m - top), w = __expf(s - top);
-        m = top;
-        l = l * old + w;
-        for (int e = 0; e < E; e++) acc[e] = __builtin_fmaf(w, (float)v[e], acc[e] * old);
-    }
-    for (int e = 0; e < E; e++) out[lane * E + e] = (TO)(n > 0 ? acc[e] / l : 0.f);
-}
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kRows = 32 * kWaves;  // query rows of a workgroup
+constexpr int kKeys = 64;           // of a tile
 
 template <int D, typename T, typename TO>
-__global__ __launch_bounds__(64) void prompt_kernel(PromptArgs a) {
-    const int t = blockIdx.x, head = blockIdx.y;
-    int lo = 0, hi = a.seqs;  // the last sequence that begins at or before t
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
+    constexpr int TB = kKeys * 2 * D, NB = kKeys / 32, GB = 16 * 2 * D;
+    constexpr bool SPLIT = sizeof(TO) == 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // [2 buffers][keys, values][64][D]
+    const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+    const int kvh = a.cache.kv_heads, G = a.q_heads / kvh;
+    // later tiles of a sequence see more keys: they go first
+    const int head = blockIdx.x % kvh, tile = tiles - 1 - blockIdx.x / kvh;
+    // sequence i's tiles begin at floor(off[i] G / 128) + i, so a tile's sequence is found without a scan
+    int lo = 0, hi = a.seqs;
+    auto offset = [&](int i) { return min(max(a.q_off[i], 0), a.tokens); };
     while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.q_off[mid] <= t) lo = mid;
+        const int mid = (lo + hi) >> 1;
+        if ((int)((int64_t)offset(mid) * G / kRows) + mid <= tile) lo = mid;
         else hi = mid;
     }
-    const int b = a.q_off[lo], e = a.q_off[lo + 1];
-    if (t < b || t >= e) return;
+    const int t0 = offset(lo), n = max(offset(lo + 1) - t0, 0);
+    const int rho0 = (tile - ((int)((int64_t)t0 * G / kRows) + lo)) * kRows;
+    const int rows = min(n * G - rho0, kRows);
+    if (rows <= 0 || rho0 < 0) return;
     const int slot = a.slots ? a.slots[lo] : lo;
-    const int64_t len = cache_length(a.cache, slot, a.kv_len[lo]);
-    const int64_t n = len - (e - b) + (t - b) + 1;
-    attend_row<D>(a.cache, static_cast<const T*>(a.q) + t * a.ldq + (int64_t)head * D, n > 0 ? slot : 0,
-                  head / (a.q_heads / a.cache.kv_heads), n, a.scale, static_cast<TO*>(a.out) + t * a.ldo + (int64_t)head * D);
+    const int len = (int)cache_length(a.cache, slot, a.kv_len[lo]);
+
+    Queries<D, T, SPLIT> w;
+    w.init();
+    const int col = wv * 32 + (lane & 31);
+    const int rho = rho0 + min(col, rows - 1);
+    const int j = rho / G, qh = head * G + rho % G;
+    const int seen = max(len - n + j + 1, 0);
+    const int first = uniform(max(len - n + (rho0 + min(wv * 32, rows - 1)) / G + 1, 0));  // seen by the wave's first row
+    const int last = uniform(max(len - n + (rho0 + min(wv * 32 + 31, rows - 1)) / G + 1, 0));
+    const int end = max(len - n + (rho0 + rows - 1) / G + 1, 0);  // keys of the workgroup
+    const float c = a.scale * kLog2e;
+
+    Loader<D> loader;
+    loader.init(a.cache, lane);
+    const int32_t* pages = a.cache.table + (int64_t)(end ? slot : 0) * a.cache.ld_table;
+    const int last_page = (max(len, 1) - 1) >> a.cache.page_bits;
+    const char* const k_base = a.cache.k + (uint64_t)head * a.cache.head_stride;
+    const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
+    auto fetch = [&](int t, int buffer) {  // each wave 16 of the tile's 64 rows
+        const uint64_t at = granule_offset(a.cache, pages, last_page, t + 16 * wv);
+        const unsigned to = lds_address(lds + buffer * 2 * TB + wv * GB);
+        loader.load(k_base + at, to);
+        loader.load(v_base + at, to + TB);
+    };
+    if (end > 0) fetch(0, 0);
+    w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
+    w.loaded();
+    int buffer = 0;
+    for (int t = 0; t < end; t += kKeys, buffer ^= 1) {
+        wait_vm<0>();
+        __syncthreads();  // the tile is there, and nobody reads the other buffer any more
+        if (t + kKeys < end) fetch(t + kKeys, buffer ^ 1);
+        if (t >= last) continue;
+        const char* kt = lds + buffer * 2 * TB;
+        f16v s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 32 * 2 * D, lane);
+        const bool part = t + kKeys > first;
+        if (part) w.hide(s, seen - t, lane);
+        w.weigh(s, c);
+        if (part) w.template add<NB, decltype(w)::kEach>(kt + TB, s, seen - t, lane);
+        else w.template add<NB, decltype(w)::kAll>(kt + TB, s, kKeys, lane);
+    }
+    w.finish_sum();
+    if (col < rows) {
+        const float r = seen > 0 ? 1.0f / w.l : 0.f;
+        using o4 = typename Vec<TO>::v4;
+        TO* out = static_cast<TO*>(a.out) + (int64_t)(t0 + j) * a.ldo + (int64_t)qh * D + 4 * (lane >> 5);
+#pragma unroll
+        for (int b = 0; b < D / 32; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<o4*>(out + 32 * b + 8 * i) =
+                    o4{(TO)(w.o[b][4 * i] * r), (TO)(w.o[b][4 * i + 1] * r), (TO)(w.o[b][4 * i + 2] * r), (TO)(w.o[b][4 * i + 3] * r)};
+    }
 }
 
 template <int D, typename T, typename TO>
 struct Prompt {
     static hipError_t go(const PromptArgs& a, hipStream_t stream) {
-        hipLaunchKernelGGL((prompt_kernel<D, T, TO>), dim3(a.tokens, a.q_heads), dim3(64), 0, stream, a);
+        constexpr int lds = 2 * 2 * kKeys * 2 * D;
+        const int G = a.q_heads / a.cache.kv_heads;
+        const int64_t tiles = (int64_t)a.tokens * G / kRows + a.seqs;
+        if (tiles * a.cache.kv_heads > INT32_MAX) return hipErrorInvalidValue;
+        static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO>),
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (ready != hipSuccess) return ready;
+        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(kThreads), lds, stream, a,
+                           (int)tiles);
         return hipGetLastError();
     }
 };
+
 }  // namespace
 
 hipError_t launch_attn_prompt(const PromptArgs& a, int dtype, int out_dtype, hipStream_t stream) {
