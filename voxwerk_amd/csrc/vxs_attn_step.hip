@@ -24,6 +24,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 32;       // query rows of a workgroup
 constexpr int kMaxParts = 256;  // of a row's keys
+constexpr int kJoin = 8;        // parts that a wave reads at once to join them
 
 // How a call's work is divided; the host and the kernel compute it from the same numbers.
 struct Split {
@@ -149,8 +150,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     constexpr bool SPLIT = sizeof(TO) == 4;
     constexpr int OS = D + 4;  // floats of a row in the join
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int kJoin = kWaves * 2 * TB > 2 * kCols * OS * 4 ? kWaves * 2 * TB : 2 * kCols * OS * 4;
-    float* wave_ml = reinterpret_cast<float*>(lds + kJoin);  // [waves][32][2]
+    constexpr int kTop = kWaves * 2 * TB > 2 * kCols * OS * 4 ? kWaves * 2 * TB : 2 * kCols * OS * 4;
+    float* wave_ml = reinterpret_cast<float*>(lds + kTop);  // [waves][32][2]
     float* sums = wave_ml + kWaves * kCols * 2;              // [32]: l of the workgroup; then the rows that are complete
     const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
     const int kvh = a.cache.kv_heads, G = sp.group;
@@ -362,25 +363,48 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         const int parts = complete[i], own = parts >> 16, all = own + (parts & 0xffff);
         if (!parts) continue;
         const int r = rbase + first + i;
-        auto part_at = [&](int p) { return p < own ? p : sq.own_parts + p - own; };
-        for (int j = threadIdx.x; j < G * (D / 4); j += kThreads) {
-            const int q = j / (D / 4), d = 4 * (j % (D / 4));
+        const bool any = cache_length(b.cache, b.slots ? b.slots[r] : r, b.kv_len[r]) > 0;
+        // A wave takes a query head at a time: a part's m and l are a lane's, then its sums are read, kJoin at once
+        // (each such read comes from the common memory), lanes along D.
+        for (int q = wv; q < G; q += kWaves) {
+            auto at = [&](int p) { return record(r, p < own ? p : sq.own_parts + p - own, q); };
+            constexpr int E = D / 128 ? D / 128 : 1;  // pairs of entries of a lane
+            const bool mine = 2 * lane < D;
             float top = kLowest, total = 0.f;
-            for (int p = 0; p < all; p++) top = fmaxf(top, get2(rec.ml + record(r, part_at(p), q) * 2).x);
-            f4 x{0.f, 0.f, 0.f, 0.f};
-            for (int p = 0; p < all; p++) {
-                const int64_t at = record(r, part_at(p), q);
-                const float2 ml = get2(rec.ml + at * 2), lo = get2(rec.o + at * D + d), hi = get2(rec.o + at * D + d + 2);
-                const float g = __builtin_amdgcn_exp2f(ml.x - top);
+            for (int p = lane; p < all; p += 64) top = fmaxf(top, get2(rec.ml + at(p) * 2).x);
+            for (int x = 32; x >= 1; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
+            float2 sum[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) sum[e] = make_float2(0.f, 0.f);
+            for (int p0 = 0; p0 < all; p0 += 64) {
+                const float2 ml = p0 + lane < all ? get2(rec.ml + at(p0 + lane) * 2) : make_float2(kLowest, 0.f);
+                const float g = p0 + lane < all ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
                 total = __builtin_fmaf(ml.y, g, total);
-                x[0] = __builtin_fmaf(lo.x, g, x[0]);
-                x[1] = __builtin_fmaf(lo.y, g, x[1]);
-                x[2] = __builtin_fmaf(hi.x, g, x[2]);
-                x[3] = __builtin_fmaf(hi.y, g, x[3]);
+                for (int p = p0; p < min(all, p0 + 64); p += kJoin) {
+                    float2 o[kJoin][E];
+#pragma unroll
+                    for (int j = 0; j < kJoin; j++)
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            o[j][e] = mine ? get2(rec.o + at(min(p + j, all - 1)) * D + 2 * (lane + 64 * e)) : make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int j = 0; j < kJoin; j++) {
+                        const float f = __shfl(g, p - p0 + j);
+                        if (p + j >= all) continue;  // (read again above)
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            sum[e].x = __builtin_fmaf(o[j][e].x, f, sum[e].x);
+                            sum[e].y = __builtin_fmaf(o[j][e].y, f, sum[e].y);
+                        }
+                    }
+                }
             }
-            const int len = (int)cache_length(b.cache, b.slots ? b.slots[r] : r, b.kv_len[r]);
-            const float y = len > 0 ? 1.0f / total : 0.f;  // (a row without keys in a group: all weights are zero)
-            *reinterpret_cast<o4*>(out_at(r, head * G + q) + d) = o4{(TO)(x[0] * y), (TO)(x[1] * y), (TO)(x[2] * y), (TO)(x[3] * y)};
+            for (int x = 32; x >= 1; x /= 2) total += __shfl_xor(total, x);
+            const float y = any ? 1.0f / total : 0.f;  // (a row without keys in a group: all weights are zero)
+            using o2 = TO __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (mine) *reinterpret_cast<o2*>(out_at(r, head * G + q) + 2 * (lane + 64 * e)) = o2{(TO)(sum[e].x * y), (TO)(sum[e].y * y)};
         }
     }
 }
