@@ -137,7 +137,7 @@ __device__ __forceinline__ A arguments_again() {
 }
 
 // Byte offset, from k or v at `head`, of the granule that begins at token t (uniform) of a slot whose table entries are
-// `pages`, the last of them that is used at `last`. Granules past the end read what is there in the pool.
+// `pages`, the last of them at `last`. Granules past a sequence's end read what is there in the pool.
 __device__ __forceinline__ uint64_t granule_offset(const PagedCache& c, const int32_t* pages, int last, int t) {
     return cache_offset(c, scalar(pages, min(t >> c.page_bits, last)), 0, t);
 }
