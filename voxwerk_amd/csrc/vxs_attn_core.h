@@ -54,6 +54,16 @@ struct Vec<float> {
     using v4 = f4;
 };
 
+// Whether one of the 8 entries of x (16 bits each) is infinite or NaN: its exponent's carry reaches the sign's place.
+template <typename T>
+__device__ __forceinline__ bool any_odd(u4 x) {
+    constexpr unsigned kOne = 0x8000u - Vec<T>::kExponent, kBoth = kOne << 16 | kOne;
+    unsigned y = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) y |= (x[i] & 0x7fff7fffu) + kBoth;
+    return (y & 0x80008000u) != 0;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {  // (a NaN loses, as in fmaxf, with nothing to canonicalise)
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -78,6 +88,15 @@ __device__ __forceinline__ void wait_vm() {  // all but the N youngest loads int
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const char* uniform_ptr(const char* p) {
+    const uint64_t x = (uint64_t)p;
+    return (const char*)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
+}
 
 template <int D>
 struct TileGeom {
@@ -104,21 +123,14 @@ struct Loader {
     }
     // base: the granule's first row (uniform); lds: where its rows go
     __device__ __forceinline__ void load(const char* base, unsigned lds) const {
+        base = uniform_ptr(base);
+        lds = uniform((int)lds);
 #pragma unroll
         for (int j = 0; j < G::kLoads; j++)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + 1024u * j), "v"(off[j]), "s"(base)
                          : "memory");
     }
 };
-
-__device__ __forceinline__ unsigned lds_address(const void* p) {
-    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
-}
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ const char* uniform_ptr(const char* p) {
-    const uint64_t x = (uint64_t)p;
-    return (const char*)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
-}
 
 // Read-only memory of the launch, read with scalar loads: they are not counted with the loads into LDS.
 template <typename A>
@@ -140,6 +152,34 @@ __device__ __forceinline__ A arguments_again() {
 // `pages`, the last of them at `last`. Granules past a sequence's end read what is there in the pool.
 __device__ __forceinline__ uint64_t granule_offset(const PagedCache& c, const int32_t* pages, int last, int t) {
     return cache_offset(c, scalar(pages, min(t >> c.page_bits, last)), 0, t);
+}
+
+// BYTES of a tile of values in LDS (whole rows, the first of which is key `row0` of the tile) before weights of zero meet
+// them: rows from `end` on, which nobody sees and which may hold anything, become zero, and with `each` so do entries
+// that are not finite, since some query does not see them; true in a lane that found such.
+template <int D, typename T, int BYTES>
+__device__ __forceinline__ bool scrub(char* rows, int row0, int end, bool each, int lane) {
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < BYTES / 1024; i++) {
+        const int at = 16 * (64 * i + lane);
+        u4* p = reinterpret_cast<u4*>(rows + at);
+        if (row0 + at / (2 * D) >= end) {
+            *p = u4{0, 0, 0, 0};
+        } else if (each) {
+            u4 x = *p;
+            if (any_odd<T>(x)) {
+                found = true;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if ((x[e] & Vec<T>::kExponent) == Vec<T>::kExponent) x[e] &= 0xffff0000u;
+                    if ((x[e] >> 16 & Vec<T>::kExponent) == Vec<T>::kExponent) x[e] &= 0xffffu;
+                }
+                *p = x;
+            }
+        }
+    }
+    return found;
 }
 
 // A wave's 32 queries: operand, running maximum, sum of its own keys' weights, and outputs O^T.
@@ -247,62 +287,36 @@ struct Queries {
         return hi;
     }
 
-    enum Mask {
-        kAll,   // every query sees every key of the tile
-        kTail,  // all queries see the same first `seen` keys: the others' values are taken as zero
-        kEach,  // each query sees its own first `seen` keys
-    };
-
-    // O^T += V^T P^T over NB x 32 keys. The weights are rounded to T once (SPLIT: the rest of each in a second product).
-    // A weight of zero does not hide an infinite or NaN value from the sum, so with kTail values past the end are
-    // zeroed, and with kEach values that are not finite are zeroed, then added for the queries that see them.
-    template <int NB, Mask MASK>
-    __device__ __forceinline__ void add(const char* tile, const f16v (&s)[NB], int seen, int lane) {
-        // (the rarer forms form their addresses anew: kept from tile to tile they would cost registers)
-        if (MASK != kAll) asm volatile("" : "+v"(lane));
+    // O^T += V^T P^T over NB x 32 keys. The weights are rounded to T once (SPLIT: the rest of each in a second product). A
+    // weight of zero hides values that are finite only: see scrub().
+    template <int NB>
+    __device__ __forceinline__ void add(const char* tile, const f16v (&s)[NB], int lane) {
         v8 hi[2 * NB], lo[2 * NB];
 #pragma unroll
         for (int k = 0; k < 2 * NB; k++) hi[k] = weights(s[k >> 1], k & 1, lo[k]);
-        unsigned odd = 0;
 #pragma unroll
         for (int b = 0; b < D / 32; b++)
 #pragma unroll
             for (int k = 0; k < 2 * NB; k++) {
-                s8 v = values(tile, k, b, lane);
-                if (MASK == kTail) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (16 * k + 8 * (e >> 2) + (e & 3) >= seen - 4 * (lane >> 5)) v[e] = 0;
-                }
-                if (MASK == kEach) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (((unsigned short)v[e] & Vec<T>::kExponent) == Vec<T>::kExponent) {
-                            v[e] = 0;
-                            odd = 1;
-                        }
-                }
-                const v8 a = __builtin_bit_cast(v8, v);
-                o[b] = Vec<T>::mfma(a, hi[k], o[b]);
-                if (SPLIT) o[b] = Vec<T>::mfma(a, lo[k], o[b]);
+                const v8 v = __builtin_bit_cast(v8, values(tile, k, b, lane));
+                o[b] = Vec<T>::mfma(v, hi[k], o[b]);
+                if (SPLIT) o[b] = Vec<T>::mfma(v, lo[k], o[b]);
             }
-        if (MASK == kEach && __ballot(odd != 0)) {
-            for (int key = 0; key < 32 * NB; key++) {
-                const char* row = tile + key * G::kRow + 8 * (lane >> 5);
-                const int sw = G::swizzle(key) << 4;
+    }
+
+    // Adds a key's values that are not finite (row: its values in memory), where this lane's query sees it.
+    __device__ __forceinline__ void add_odd(const char* row, bool sees, int lane) {
+        row += 8 * (lane >> 5);
 #pragma unroll
-                for (int b = 0; b < D / 32; b++)
+        for (int b = 0; b < D / 32; b++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const s4 x = *reinterpret_cast<const s4*>(row + ((64 * b + 16 * j) ^ sw));
+            for (int j = 0; j < 4; j++) {
+                const s4 x = *reinterpret_cast<const s4*>(row + 64 * b + 16 * j);
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (((unsigned short)x[e] & Vec<T>::kExponent) == Vec<T>::kExponent && key < seen)
-                                o[b][4 * j + e] += (float)__builtin_bit_cast(T, (short)x[e]);
-                        asm volatile("" ::: "memory");  // (one read at a time: this may be slow, not large)
-                    }
+                for (int e = 0; e < 4; e++)
+                    if (((unsigned short)x[e] & Vec<T>::kExponent) == Vec<T>::kExponent && sees)
+                        o[b][4 * j + e] += (float)__builtin_bit_cast(T, (short)x[e]);
             }
-        }
     }
 
     __device__ __forceinline__ void finish_sum() { l += __shfl_xor(l, 32); }

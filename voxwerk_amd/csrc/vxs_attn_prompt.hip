@@ -32,20 +32,25 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel
     const int kvh = a.cache.kv_heads, G = a.q_heads / kvh;
     // later tiles of a sequence see more keys: they go first
     const int head = blockIdx.x % kvh, tile = tiles - 1 - blockIdx.x / kvh;
-    // sequence i's tiles begin at floor(off[i] G / 128) + i, so a tile's sequence is found without a scan
-    int lo = 0, hi = a.seqs;
-    auto offset = [&](int i) { return min(max(a.q_off[i], 0), a.tokens); };
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((int)((int64_t)offset(mid) * G / kRows) + mid <= tile) lo = mid;
-        else hi = mid;
+    // Sequence i's tiles begin at floor(off[i] G / 128) + i, so a tile's sequence is found without a scan: the last that
+    // begins at or before it, 64 of them in one read.
+    int seq = 0, t0 = 0, n = 0;
+    auto begin = [&](int off, int i) { return (int)((int64_t)off * G / kRows) + i; };
+    for (int i0 = 0; i0 < a.seqs; i0 += 64) {
+        const int i = min(i0 + lane, a.seqs - 1);
+        const int off = min(max(a.q_off[i], 0), a.tokens), next = min(max(a.q_off[i + 1], off), a.tokens);
+        const uint64_t before = __ballot(i0 + lane < a.seqs && begin(off, i) <= tile);
+        if (!before) break;
+        const int at = 63 - __builtin_clzll(before);
+        seq = i0 + at;
+        t0 = __builtin_amdgcn_readlane(off, at);
+        n = __builtin_amdgcn_readlane(next, at) - t0;
     }
-    const int t0 = offset(lo), n = max(offset(lo + 1) - t0, 0);
-    const int rho0 = (tile - ((int)((int64_t)t0 * G / kRows) + lo)) * kRows;
+    const int rho0 = (tile - begin(t0, seq)) * kRows;
     const int rows = min(n * G - rho0, kRows);
     if (rows <= 0 || rho0 < 0) return;
-    const int slot = a.slots ? a.slots[lo] : lo;
-    const int len = (int)cache_length(a.cache, slot, a.kv_len[lo]);
+    const int slot = a.slots ? scalar(a.slots, seq) : seq;
+    const int len = (int)cache_length(a.cache, slot, scalar(a.kv_len, seq));
 
     Queries<D, T, SPLIT> w;
     w.init();
@@ -61,7 +66,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel
     Loader<D> loader;
     loader.init(a.cache, lane);
     const int32_t* pages = a.cache.table + (int64_t)(end ? slot : 0) * a.cache.ld_table;
-    const int last_page = (max(len, 1) - 1) >> a.cache.page_bits;
+    const int last_page = (int)a.cache.ld_table - 1;
     const char* const k_base = a.cache.k + (uint64_t)head * a.cache.head_stride;
     const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
     auto fetch = [&](int t, int buffer) {  // each wave 16 of the tile's 64 rows
@@ -73,21 +78,31 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel
     if (end > 0) fetch(0, 0);
     w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
     w.loaded();
+    const int all = uniform(max(len - n + rho0 / G + 1, 0));  // keys that every row of the workgroup sees
+    bool odd = false;
     int buffer = 0;
     for (int t = 0; t < end; t += kKeys, buffer ^= 1) {
         wait_vm<0>();
         __syncthreads();  // the tile is there, and nobody reads the other buffer any more
         if (t + kKeys < end) fetch(t + kKeys, buffer ^ 1);
+        char* const kt = lds + buffer * 2 * TB;
+        if (t + kKeys > all) {  // some row does not see all of the tile: each wave looks through a quarter of the values
+            odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
+            __syncthreads();
+        }
         if (t >= last) continue;
-        const char* kt = lds + buffer * 2 * TB;
         f16v s[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 32 * 2 * D, lane);
-        const bool part = t + kKeys > first;
-        if (part) w.hide(s, seen - t, lane);
+        if (t + kKeys > first) w.hide(s, seen - t, lane);
         w.weigh(s, c);
-        if (part) w.template add<NB, decltype(w)::kEach>(kt + TB, s, seen - t, lane);
-        else w.template add<NB, decltype(w)::kAll>(kt + TB, s, kKeys, lane);
+        w.add(kt + TB, s, lane);
+    }
+    if (__syncthreads_or(odd)) {
+        for (int t = all & ~(kKeys - 1); t < end; t++)
+            w.add_odd(a.cache.v + (uint64_t)head * a.cache.head_stride + granule_offset(a.cache, pages, last_page, t & ~15) +
+                          (uint64_t)(t & 15) * a.cache.token_stride,
+                      t < seen, lane);
     }
     w.finish_sum();
     if (col < rows) {

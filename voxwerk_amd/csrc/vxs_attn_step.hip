@@ -271,6 +271,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     }
     const float c = a.scale * kLog2e;
     w.loaded();
+    bool odd = false;
     for (; t < c1; t += step) {
         const bool more = t + step < c1;
         if (more) find(t + step);
@@ -285,15 +286,21 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         w.weigh(s, c);
         if (more) wait_vm<NI>();
         else wait_vm<0>();
-        if (each) w.template add<NB, decltype(w)::kEach>(vt, s, seen - t, lane);
-        else if (tail) w.template add<NB, decltype(w)::kTail>(vt, s, c1 - t, lane);
-        else w.template add<NB, decltype(w)::kAll>(vt, s, KT, lane);
+        if (each || tail) odd |= scrub<D, T, TB>(vt, t, c1, each, lane);
+        w.add(vt, s, lane);
         wait_lds();
         if (more) fetch(v_base, v_lds);
     }
     w.finish_sum();
     const KernelArgs again = arguments_again<KernelArgs>();
     const StepArgs& b = again.a;
+    if (each && __ballot(odd)) {
+        for (t = c0 + wv * KT; t < c1; t += t % KT == KT - 1 ? step - KT + 1 : 1)
+            w.add_odd(b.cache.v + (uint64_t)head * b.cache.head_stride +
+                          granule_offset(b.cache, b.cache.table + (int64_t)slot * b.cache.ld_table, (int)b.cache.ld_table - 1, t & ~15) +
+                          (uint64_t)(t & 15) * b.cache.token_stride,
+                      t < seen, lane);
+    }
     const Split& sq = again.sp;
     const Records& rec = again.rec;
 
