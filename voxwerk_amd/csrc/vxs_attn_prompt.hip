@@ -6,8 +6,9 @@
 //
 // Bound by the matrix cores: 4 D operations for each query head and key that it sees. The query heads of one key head
 // are stacked, row rho = j G + g for token j and head g of G, so all rows of a workgroup read the same keys: a wave
-// holds 32 rows (vxs_attn_core.h), the four waves of a workgroup 128 consecutive ones, and each tile of 64 keys is loaded
-// into LDS once for all four, the next one while this one is used.
+// holds 32 rows (vxs_attn_core.h), QW waves 32 QW consecutive ones, and each tile of keys is loaded into LDS once for
+// all of them, the next one while this one is used. Where that leaves compute units idle, KW such groups of waves take a
+// workgroup's tiles in turn, and their sums are joined through LDS at the end.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -18,21 +19,28 @@
 namespace vxs {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;  // query rows of a workgroup
-constexpr int kKeys = 64;           // of a tile
+template <int D, int QW, int KW>
+struct Shape {
+    static constexpr int kThreads = 64 * QW * KW;
+    static constexpr int kRows = 32 * QW;    // query rows of a workgroup
+    static constexpr int kKeys = 16 * QW;    // of a tile: each wave loads a granule of 16
+    static constexpr int kTile = kKeys * 2 * D;
+    static constexpr int kTiles = KW * 4 * kTile;                             // [groups][2 buffers][keys, values]
+    static constexpr int kSums = KW == 1 ? 0 : QW * KW * 32 * (D + 4 + 2) * 4;  // [waves][32][D + 4], [waves][32] m and l
+    static constexpr int kLds = kTiles > kSums ? kTiles : kSums;
+};
 
-template <int D, typename T, typename TO>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
-    constexpr int TB = kKeys * 2 * D, NB = kKeys / 32, GB = 16 * 2 * D;
+template <int D, typename T, typename TO, int QW, int KW>
+__global__ __launch_bounds__(64 * QW * KW, D == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
+    using S = Shape<D, QW, KW>;
+    constexpr int TB = S::kTile, NB = S::kKeys / 32, GB = 16 * 2 * D, kRows = S::kRows, kKeys = S::kKeys;
     constexpr bool SPLIT = sizeof(TO) == 4;
-    extern __shared__ __attribute__((aligned(16))) char lds[];  // [2 buffers][keys, values][64][D]
-    const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wv = wave % QW, kg = wave / QW;
     const int kvh = a.cache.kv_heads, G = a.q_heads / kvh;
     // later tiles of a sequence see more keys: they go first
     const int head = blockIdx.x % kvh, tile = tiles - 1 - blockIdx.x / kvh;
-    // Sequence i's tiles begin at floor(off[i] G / 128) + i, so a tile's sequence is found without a scan: the last that
+    // Sequence i's tiles begin at floor(off[i] G / kRows) + i, so a tile's sequence is found without a scan: the last that
     // begins at or before it, 64 of them in one read.
     int seq = 0, t0 = 0, n = 0;
     auto begin = [&](int off, int i) { return (int)((int64_t)off * G / kRows) + i; };
@@ -60,7 +68,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel
     const int seen = max(len - n + j + 1, 0);
     const int first = uniform(max(len - n + (rho0 + min(wv * 32, rows - 1)) / G + 1, 0));  // seen by the wave's first row
     const int last = uniform(max(len - n + (rho0 + min(wv * 32 + 31, rows - 1)) / G + 1, 0));
-    const int end = max(len - n + (rho0 + rows - 1) / G + 1, 0);  // keys of the workgroup
+    const int all = uniform(max(len - n + rho0 / G + 1, 0));               // keys that every row of the workgroup sees
+    const int end = uniform(max(len - n + (rho0 + rows - 1) / G + 1, 0));  // that some row sees
     const float c = a.scale * kLog2e;
 
     Loader<D> loader;
@@ -69,25 +78,26 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel
     const int last_page = (int)a.cache.ld_table - 1;
     const char* const k_base = a.cache.k + (uint64_t)head * a.cache.head_stride;
     const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
-    auto fetch = [&](int t, int buffer) {  // each wave 16 of the tile's 64 rows
+    char* const own = lds + kg * 4 * TB;
+    auto fetch = [&](int t, int buffer) {  // each wave 16 of the tile's rows
         const uint64_t at = granule_offset(a.cache, pages, last_page, t + 16 * wv);
-        const unsigned to = lds_address(lds + buffer * 2 * TB + wv * GB);
+        const unsigned to = lds_address(own + buffer * 2 * TB + wv * GB);
         loader.load(k_base + at, to);
         loader.load(v_base + at, to + TB);
     };
-    if (end > 0) fetch(0, 0);
+    if (kg * kKeys < end) fetch(kg * kKeys, 0);
     w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
     w.loaded();
-    const int all = uniform(max(len - n + rho0 / G + 1, 0));  // keys that every row of the workgroup sees
     bool odd = false;
     int buffer = 0;
-    for (int t = 0; t < end; t += kKeys, buffer ^= 1) {
+    for (int base = 0; base < end; base += KW * kKeys, buffer ^= 1) {
+        const int t = base + kg * kKeys;
         wait_vm<0>();
-        __syncthreads();  // the tile is there, and nobody reads the other buffer any more
-        if (t + kKeys < end) fetch(t + kKeys, buffer ^ 1);
-        char* const kt = lds + buffer * 2 * TB;
-        if (t + kKeys > all) {  // some row does not see all of the tile: each wave looks through a quarter of the values
-            odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
+        __syncthreads();  // the tiles are there, and nobody reads the other buffers any more
+        if (t + KW * kKeys < end) fetch(t + KW * kKeys, buffer ^ 1);
+        char* const kt = own + buffer * 2 * TB;
+        if (base + KW * kKeys > all) {  // some row does not see all of the tiles: each wave looks through its part of the values
+            if (t < end) odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
             __syncthreads();
         }
         if (t >= last) continue;
@@ -99,38 +109,79 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_prompt_kernel
         w.add(kt + TB, s, lane);
     }
     if (__syncthreads_or(odd)) {
-        for (int t = all & ~(kKeys - 1); t < end; t++)
-            w.add_odd(a.cache.v + (uint64_t)head * a.cache.head_stride + granule_offset(a.cache, pages, last_page, t & ~15) +
-                          (uint64_t)(t & 15) * a.cache.token_stride,
-                      t < seen, lane);
+        for (int t = all / (KW * kKeys) * (KW * kKeys); t < end; t++)  // (the tiles that were looked through)
+            if (KW == 1 || t / kKeys % KW == kg)
+                w.add_odd(v_base + granule_offset(a.cache, pages, last_page, t & ~15) + (uint64_t)(t & 15) * a.cache.token_stride, t < seen, lane);
     }
     w.finish_sum();
-    if (col < rows) {
-        const float r = seen > 0 ? 1.0f / w.l : 0.f;
-        using o4 = typename Vec<TO>::v4;
-        TO* out = static_cast<TO*>(a.out) + (int64_t)(t0 + j) * a.ldo + (int64_t)qh * D + 4 * (lane >> 5);
+    using o4 = typename Vec<TO>::v4;
+    if (KW == 1) {
+        if (col < rows) {
+            const float r = seen > 0 ? 1.0f / w.l : 0.f;
+            TO* out = static_cast<TO*>(a.out) + (int64_t)(t0 + j) * a.ldo + (int64_t)qh * D + 4 * (lane >> 5);
 #pragma unroll
-        for (int b = 0; b < D / 32; b++)
+            for (int b = 0; b < D / 32; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                *reinterpret_cast<o4*>(out + 32 * b + 8 * i) =
-                    o4{(TO)(w.o[b][4 * i] * r), (TO)(w.o[b][4 * i + 1] * r), (TO)(w.o[b][4 * i + 2] * r), (TO)(w.o[b][4 * i + 3] * r)};
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<o4*>(out + 32 * b + 8 * i) =
+                        o4{(TO)(w.o[b][4 * i] * r), (TO)(w.o[b][4 * i + 1] * r), (TO)(w.o[b][4 * i + 2] * r), (TO)(w.o[b][4 * i + 3] * r)};
+        }
+        return;
+    }
+    // (the barrier above: every wave is done with its tiles)
+    constexpr int OS = D + 4;
+    float* const sums = reinterpret_cast<float*>(lds);
+    float* const ml = sums + QW * KW * 32 * OS;
+#pragma unroll
+    for (int b = 0; b < D / 32; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *reinterpret_cast<f4*>(sums + (wave * 32 + (lane & 31)) * OS + 32 * b + 8 * i + 4 * (lane >> 5)) =
+                f4{w.o[b][4 * i], w.o[b][4 * i + 1], w.o[b][4 * i + 2], w.o[b][4 * i + 3]};
+    if (lane < 32) *reinterpret_cast<float2*>(ml + (wave * 32 + lane) * 2) = make_float2(w.m, w.l);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (D / 4); i += S::kThreads) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));  // row r is column r % 32 of waves r / 32 + QW * group
+        float m = kLowest, l = 0.f;
+#pragma unroll
+        for (int g = 0; g < KW; g++) m = fmaxf(m, ml[(g * QW * 32 + r) * 2]);
+        f4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < KW; g++) {
+            const float2 x = *reinterpret_cast<const float2*>(ml + (g * QW * 32 + r) * 2);
+            const float f = __builtin_amdgcn_exp2f(x.x - m);
+            l = __builtin_fmaf(x.y, f, l);
+            o = o + *reinterpret_cast<const f4*>(sums + (g * QW * 32 + r) * OS + d) * f;
+        }
+        const int jr = (rho0 + r) / G, h = head * G + (rho0 + r) % G;
+        const float y = len - n + jr + 1 > 0 ? 1.0f / l : 0.f;
+        *reinterpret_cast<o4*>(static_cast<TO*>(a.out) + (int64_t)(t0 + jr) * a.ldo + (int64_t)h * D + d) =
+            o4{(TO)(o[0] * y), (TO)(o[1] * y), (TO)(o[2] * y), (TO)(o[3] * y)};
     }
 }
 
 template <int D, typename T, typename TO>
 struct Prompt {
-    static hipError_t go(const PromptArgs& a, hipStream_t stream) {
-        constexpr int lds = 2 * 2 * kKeys * 2 * D;
-        const int G = a.q_heads / a.cache.kv_heads;
-        const int64_t tiles = (int64_t)a.tokens * G / kRows + a.seqs;
+    template <int QW, int KW>
+    static hipError_t launch(const PromptArgs& a, hipStream_t stream) {
+        using S = Shape<D, QW, KW>;
+        const int64_t tiles = tiles_of(a, S::kRows);
         if (tiles * a.cache.kv_heads > INT32_MAX) return hipErrorInvalidValue;
-        static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO>),
-                                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW>),
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
         if (ready != hipSuccess) return ready;
-        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(kThreads), lds, stream, a,
-                           (int)tiles);
+        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,
+                           a, (int)tiles);
         return hipGetLastError();
+    }
+    static int64_t tiles_of(const PromptArgs& a, int rows) { return (int64_t)a.tokens * (a.q_heads / a.cache.kv_heads) / rows + a.seqs; }
+    static hipError_t go(const PromptArgs& a, hipStream_t stream) {
+        // Four groups of two waves (two at D = 256, for the LDS) while 128 rows a workgroup leave compute units idle and a cache
+        // may hold more than a few tiles (us, groups / 128 rows: one prompt of 1000 18.8 / 25.5, of 2000, 264 workgroups, 37 / 45,
+        // 4 of 500 to 1000, 408 workgroups, 43 / 27; 130 tokens after 8000 91 / 162; one of 93 9.5 / 7.9).
+        if (tiles_of(a, 128) * a.cache.kv_heads <= 288 && (a.cache.ld_table << a.cache.page_bits) > 256)
+            return launch<2, D == 256 ? 2 : 4>(a, stream);
+        return launch<4, 1>(a, stream);
     }
 };
 
