@@ -425,6 +425,7 @@ typedef struct vxs_shared_prefix {
  * (d_slots[r]; NULL: slot r), its own among them. Results, types and layouts as vxs_attn_prompt_device; a row of
  * length 0 gets zeros. max_len: no length is longer (the work is divided for it; a longer one costs time, not
  * correctness). prefix: NULL, or the rows' shared prefixes.
+ * A few new tokens of one long sequence can be rows too: the same slot, a length each, their context as a shared prefix.
  *
  * work: device memory of vxs_attn_step_workspace bytes, 16-byte aligned, zeroed once before its first use; calls
  * leave it ready for the next. One call at a time may use it (calls on one stream are in order). NULL: each row's keys

@@ -363,3 +363,16 @@ def test_refusals(ctx):
     prompt(tokens=0)
     prompt(seqs=0)
     ctx.synchronize()
+
+
+def test_step_rows_of_one_sequence(ctx):
+    """A few new tokens of a long sequence as rows of a step: one slot, a row's own length each, their context shared."""
+    n, new = 1500, 9
+    paged = Paged([n, 70], 2, 128, 16, "bf16", seed=4)
+    q = rows_of(new, 8, 128, "bf16", paged.rng, scale=2.0)
+    lens = [n - new + 1 + i for i in range(new)]
+    context = n - new
+    got = run_step(ctx, paged, q, 8, 0.1, "f32", kv_len=lens, slots=[0] * new, share=[(0, new, context)])
+    check(got, q, lens, lambda r, h: paged.entries(0, lens[r], h), 8, 2, 128, 0.1, "bf16", "f32", "rows of one sequence")
+    whole = run_prompt(ctx, paged, q, [0, new], 8, 0.1, "f32", kv_len=[n], slots=[0])
+    assert np.linalg.norm(whole - got) <= 2e-5 * np.linalg.norm(got)
