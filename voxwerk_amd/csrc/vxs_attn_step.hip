@@ -24,7 +24,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 32;       // query rows of a workgroup
 constexpr int kMaxParts = 256;  // of a row's keys
-constexpr int kAtOnce = 8;      // parts that a lane reads at once to join them
+constexpr int kAtOnce = 8;      // parts that are asked for at once to join them
 
 template <int D>
 constexpr int kTile = D == 64 ? 64 : 32;  // keys of a wave's tile: 8 KiB of keys, 16 at D = 256
@@ -106,16 +106,20 @@ struct Records {
     int parts;
 };
 int64_t records_counts(int rows, int kv_heads) { return ((int64_t)rows * kv_heads + 3) / 4 * 4; }
+int64_t records_ml(int rows, int q_heads, int parts) { return ((int64_t)rows * q_heads * parts * 2 + 3) / 4 * 4; }  // (what follows is 16-byte aligned)
 
 int64_t work_bytes(const StepArgs& a, const Split& s) {
     const int parts = s.own_parts + s.pre_parts;
     if (parts <= 1) return 0;
-    return 4 * (records_counts(a.rows, a.cache.kv_heads) + (int64_t)a.rows * a.q_heads * parts * (a.cache.head_dim + 2));
+    return 4 * (records_counts(a.rows, a.cache.kv_heads) + records_ml(a.rows, a.q_heads, parts) + (int64_t)a.rows * a.q_heads * parts * a.cache.head_dim);
 }
 
 __device__ __forceinline__ void put2(float* p, float a, float b) {
     const uint64_t x = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
     __hip_atomic_store(reinterpret_cast<uint64_t*>(p), x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put4(float* p, f4 x) {  // (16-byte aligned; the wait for it is the caller's)
+    asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(x) : "memory");
 }
 __device__ __forceinline__ float2 get2(const float* p) {
     const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -352,8 +356,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         const f4 x = joined(q, d4);
         const int up = pre ? sq.group.div(rho0 + q) : 0;
         const int64_t to = record(rbase + up, pre ? sq.own_parts + part : part, rho0 + q - up * G);
-        put2(rec.o + to * D + d4, x[0], x[1]);
-        put2(rec.o + to * D + d4 + 2, x[2], x[3]);
+        put4(rec.o + to * D + d4, x);
         if (d4 == 0) put2(rec.ml + to * 2, m, l);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -373,47 +376,62 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         if (!solo) complete[tid] = mine;
     }
     sync();
-    // L lanes take a (row, query head) whose row is complete: the parts' m and l are read one by a lane, their sums
-    // kAtOnce parts at a time (each read is one of the common memory).
-    const int sub = lane & (L - 1);
-    for (int pair = tid / L; pair < rows * G; pair += threads / L) {
-        const int i = sq.group.div(pair), q = pair - i * G, r = rbase + first + i;
-        const int what = solo ? uniform(mine) : complete[i], own = (what >> 15) & 0x7fff, all = own + (what & 0x7fff);
-        if (what) {
-            auto at = [&](int p) { return record(r, p < own ? p : sq.own_parts + p - own, q); };
-            float top = kLowest;
-            for (int p = sub; p < all; p += L) top = fmaxf(top, get2(rec.ml + at(p) * 2).x);
+    // L lanes take a (row, query head) whose row is complete, four entries each, two of them at a time: kAtOnce parts are asked for
+    // together (each read is one of the common memory) and joined lane by lane.
+    const int sub = tid % L, apart = threads / L;
+    for (int pair0 = tid / L; pair0 < rows * G; pair0 += 2 * apart) {
+        float2 ml[2][kAtOnce], lo[2][kAtOnce], hi[2][kAtOnce];
+        int what[2], own[2], all[2], row[2], q[2];
+        auto fetch_parts = [&](int u, int p0) {
 #pragma unroll
-            for (int x = L / 2; x >= 1; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
+            for (int j = 0; j < kAtOnce; j++) {
+                const int p = p0 + j;
+                ml[u][j] = make_float2(kLowest, 0.f);
+                lo[u][j] = hi[u][j] = make_float2(0.f, 0.f);
+                if (p >= all[u]) continue;
+                const int64_t at = record(row[u], p < own[u] ? p : sq.own_parts + p - own[u], q[u]);
+                ml[u][j] = get2(rec.ml + at * 2);
+                lo[u][j] = get2(rec.o + at * D + 4 * sub);
+                hi[u][j] = get2(rec.o + at * D + 4 * sub + 2);
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int pair = pair0 + u * apart;
+            const int i = sq.group.div(min(pair, rows * G - 1));
+            q[u] = pair - i * G;
+            row[u] = rbase + first + i;
+            what[u] = pair < rows * G ? (solo ? uniform(mine) : complete[i]) : 0;
+            own[u] = (what[u] >> 15) & 0x7fff;
+            all[u] = own[u] + (what[u] & 0x7fff);
+            fetch_parts(u, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float top = kLowest, total = 0.f;
             f4 sum{0.f, 0.f, 0.f, 0.f};
-            float total = 0.f;
-            for (int p0 = 0; p0 < all; p0 += L) {
-                const float2 ml = p0 + sub < all ? get2(rec.ml + at(p0 + sub) * 2) : make_float2(kLowest, 0.f);
-                const float g = p0 + sub < all ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
-                total = __builtin_fmaf(ml.y, g, total);
-                for (int p = p0; p < min(all, p0 + L); p += kAtOnce) {
-                    float2 lo[kAtOnce], hi[kAtOnce];
+            for (int p = 0; p < all[u]; p += kAtOnce) {
+                if (p) fetch_parts(u, p);
+                float next = top;
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; j++) {
-                        const float* from = rec.o + at(min(p + j, all - 1)) * D + 4 * sub;
-                        lo[j] = get2(from);
-                        hi[j] = get2(from + 2);
-                    }
+                for (int j = 0; j < kAtOnce; j++) next = fmaxf(next, ml[u][j].x);
+                const float shrink = __builtin_amdgcn_exp2f(top - next);
+                top = next;
+                total *= shrink;
+                sum = sum * shrink;
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; j++) {
-                        const float f = __shfl(g, (lane & ~(L - 1)) + ((p - p0 + j) & (L - 1)));
-                        if (p + j >= all) continue;  // (read again above)
-                        sum[0] = __builtin_fmaf(lo[j].x, f, sum[0]);
-                        sum[1] = __builtin_fmaf(lo[j].y, f, sum[1]);
-                        sum[2] = __builtin_fmaf(hi[j].x, f, sum[2]);
-                        sum[3] = __builtin_fmaf(hi[j].y, f, sum[3]);
-                    }
+                for (int j = 0; j < kAtOnce; j++) {
+                    const float g = __builtin_amdgcn_exp2f(ml[u][j].x - top);  // (a part that is not there adds zeros)
+                    total = __builtin_fmaf(ml[u][j].y, g, total);
+                    sum[0] = __builtin_fmaf(lo[u][j].x, g, sum[0]);
+                    sum[1] = __builtin_fmaf(lo[u][j].y, g, sum[1]);
+                    sum[2] = __builtin_fmaf(hi[u][j].x, g, sum[2]);
+                    sum[3] = __builtin_fmaf(hi[u][j].y, g, sum[3]);
                 }
             }
-#pragma unroll
-            for (int x = L / 2; x >= 1; x /= 2) total += __shfl_xor(total, x);
-            const float y = what >> 30 ? 1.0f / total : 0.f;  // (a row without keys in a group: all weights are zero)
-            *reinterpret_cast<o4*>(out_at(r, head * G + q) + 4 * sub) = o4{(TO)(sum[0] * y), (TO)(sum[1] * y), (TO)(sum[2] * y), (TO)(sum[3] * y)};
+            const float y = what[u] >> 30 ? 1.0f / total : 0.f;  // (a row without keys in a group: all weights are zero)
+            if (what[u])
+                *reinterpret_cast<o4*>(out_at(row[u], head * G + q[u]) + 4 * sub) = o4{(TO)(sum[0] * y), (TO)(sum[1] * y), (TO)(sum[2] * y), (TO)(sum[3] * y)};
         }
     }
 }
@@ -427,7 +445,7 @@ struct Step {
         if (a.work) {
             r.count = static_cast<unsigned*>(a.work);
             r.ml = static_cast<float*>(a.work) + records_counts(a.rows, a.cache.kv_heads);
-            r.o = r.ml + (int64_t)a.rows * a.q_heads * r.parts * 2;
+            r.o = r.ml + records_ml(a.rows, a.q_heads, r.parts);
         }
         const int64_t own = (int64_t)a.rows * a.cache.kv_heads * s.head_tiles * s.own_parts;
         const int64_t blocks = (int64_t)s.pre_tiles * s.pre_parts * a.cache.kv_heads + (s.solo ? (own + kWaves - 1) / kWaves : own);
