@@ -325,6 +325,9 @@ VXS_API int vxs_frame_embed_device(vxs_ctx* ctx, int rows, int groups, int hidde
 #define VXS_BF16 1
 #define VXS_F16 2
 
+/* flag of vxs_shared_prefix */
+#define VXS_FLAG_SHARE_ALWAYS (1u << 12)
+
 /*
  * One layer's cache: keys and values of `pages` pages of `page_size` tokens each. Token t of slot s
  * (a sequence) lies in page p = table[s * ld_table + t / page_size], its key of head h at
@@ -409,15 +412,16 @@ VXS_API int vxs_attn_prompt_device(vxs_ctx* ctx, int seqs, int tokens, int q_hea
 
 /*
  * A prefix that groups of rows share (the same voice or instructions): rows [d_off[g], d_off[g + 1]) hold the same
- * pages, or copies of the same entries, for their first d_len[g] tokens, which are read once for all of them, from the
- * first row's pages. d_off int32 [groups + 1] (ascending) and d_len int32 [groups] in device memory; max_len: no
- * d_len is longer. Rows outside every group share nothing.
+ * pages, or copies of the same entries, for their first d_len[g] tokens. Those are read once for all of them, from the
+ * first row's pages, where that is faster than each row's reading its own. d_off int32 [groups + 1] (ascending) and d_len
+ * int32 [groups] in device memory; max_len: no d_len is longer. Rows outside every group share nothing.
  */
 typedef struct vxs_shared_prefix {
     const int32_t* d_off;
     const int32_t* d_len;
     int32_t groups;
     int32_t max_len;
+    uint32_t flags; /* VXS_FLAG_NONE, or VXS_FLAG_SHARE_ALWAYS: also where each row's reading its own is faster */
 } vxs_shared_prefix;
 
 /*

@@ -109,7 +109,7 @@ def as_out(x, out_dtype):
 
 
 def run_step(ctx, paged, q, q_heads, scale, out_dtype="f32", kv_len=None, slots=None, share=(), max_len=None, work="own",
-             ldo_pad=0, groups=None):
+             ldo_pad=0, always=True):
     """One step over `paged`; returns the outputs [rows, q_heads * dim + ldo_pad]."""
     rows = len(q)
     kv_len = paged.lens if kv_len is None else kv_len
@@ -117,7 +117,7 @@ def run_step(ctx, paged, q, q_heads, scale, out_dtype="f32", kv_len=None, slots=
     if share:
         off = [share[0][0]] + [hi for _, hi, _ in share]
         keep = device(np.array(off, np.int32)), device(np.array([n for *_, n in share], np.int32))
-        prefix = SharedPrefix(len(share), *keep, max(n for *_, n in share))
+        prefix = SharedPrefix(len(share), *keep, max(n for *_, n in share), always)
     ldo = q_heads * paged.dim + ldo_pad
     out, dq = out_array(rows, ldo, out_dtype), device(q)
     max_len = max(max(kv_len, default=0), 0) if max_len is None else max_len

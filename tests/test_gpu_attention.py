@@ -161,7 +161,7 @@ def test_step_workspace_is_ready_again(ctx):
     share = [(0, 24, 500)]
     shared = Paged([700] * 24, 2, 128, 16, seed=3, share=share)
     n = max(ctx.attn_step_workspace(2, 8, long.cache, 2900), ctx.attn_step_workspace(24, 8, wide.cache, 700),
-            ctx.attn_step_workspace(24, 8, shared.cache, 700, SharedPrefix(1, 16, 16, 500)))
+            ctx.attn_step_workspace(24, 8, shared.cache, 700, SharedPrefix(1, 16, 16, 500, True)))
     work = device(np.zeros(n, np.uint8))
     qs = [rows_of(len(p.lens), 8, 128, "bf16", p.rng, scale=2.0) for p in (long, wide, shared)]
     first = None
@@ -352,6 +352,9 @@ def test_refusals(ctx):
     refused(bad, step, prefix=SharedPrefix(1, None, i32, 4))
     refused(bad, step, prefix=SharedPrefix(1, i32, None, 4))
     refused(bad, step, prefix=SharedPrefix(1, i32, i32, -4))
+    odd = SharedPrefix(1, i32, i32, 4)
+    odd.struct.flags = 1
+    refused(bad, step, prefix=odd)
     refused(bad, step, workspace=x.ptr + 4, workspace_bytes=1 << 16)
     n = ctx.attn_step_workspace(1, 4, cache(), 1 << 20)
     assert n >= 0
@@ -376,3 +379,11 @@ def test_step_rows_of_one_sequence(ctx):
     check(got, q, lens, lambda r, h: paged.entries(0, lens[r], h), 8, 2, 128, 0.1, "bf16", "f32", "rows of one sequence")
     whole = run_prompt(ctx, paged, q, [0, new], 8, 0.1, "f32", kv_len=[n], slots=[0])
     assert np.linalg.norm(whole - got) <= 2e-5 * np.linalg.norm(got)
+
+
+@pytest.mark.parametrize("rows,prefix", [(6, 90), (70, 900)])
+def test_step_shares_where_it_is_faster(ctx, rows, prefix):
+    """Without the flag a prefix is shared from some size on; either way the outputs are the rows' own."""
+    share = [(0, rows, prefix)]
+    paged = Paged([prefix + 1 + i % 37 for i in range(rows)], 8, 128, 16, "bf16", seed=rows, share=share)
+    step_and_check(ctx, paged, 16, "f32", share=share, always=False)

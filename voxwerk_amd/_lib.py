@@ -31,6 +31,7 @@ VXS_FLAG_PATH_BLOCK = 1 << 8
 VXS_FLAG_PATH_WAVE = 1 << 9
 VXS_FLAG_RNG_TALKER = 1 << 10
 VXS_FLAG_RNG_SUB = 1 << 11
+VXS_FLAG_SHARE_ALWAYS = 1 << 12
 VXS_F32, VXS_BF16, VXS_F16 = 0, 1, 2
 
 
@@ -98,7 +99,7 @@ class VxsKvPrep(ctypes.Structure):
 class VxsSharedPrefix(ctypes.Structure):
     """vxs_shared_prefix (include/vxs_sampler.h)."""
 
-    _fields_ = [("d_off", c_void_p), ("d_len", c_void_p), ("groups", c_int32), ("max_len", c_int32)]
+    _fields_ = [("d_off", c_void_p), ("d_len", c_void_p), ("groups", c_int32), ("max_len", c_int32), ("flags", c_uint32)]
 
 
 _P = c_void_p  # raw pointers are passed as integers / c_void_p

@@ -50,11 +50,12 @@ class KvPrep:
 
 class SharedPrefix:
     """Groups of rows whose first tokens are the same (vxs_shared_prefix): rows [off[g], off[g + 1]) share their
-    first len[g] <= max_len tokens; `off` int32 [groups + 1], `length` int32 [groups], device memory."""
+    first len[g] <= max_len tokens; `off` int32 [groups + 1], `length` int32 [groups], device memory. They are read once for
+    a group where that is faster, with `always` in any case."""
 
-    def __init__(self, groups: int, off, length, max_len: int):
+    def __init__(self, groups: int, off, length, max_len: int, always: bool = False):
         self._keep = (off, length)
-        self.struct = _lib.VxsSharedPrefix(ptr(off), ptr(length), groups, max_len)
+        self.struct = _lib.VxsSharedPrefix(ptr(off), ptr(length), groups, max_len, _lib.VXS_FLAG_SHARE_ALWAYS if always else 0)
         self.ref = ctypes.byref(self.struct)
 
 

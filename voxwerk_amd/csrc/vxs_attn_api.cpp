@@ -77,6 +77,7 @@ int step_args(vxs_ctx* ctx, int rows, int q_heads, const vxs_kv_cache* cache, in
     a.max_len = max_len;
     a.prefix = vxs_shared_prefix{};
     if (prefix) {
+        if (prefix->flags & ~VXS_FLAG_SHARE_ALWAYS) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "unknown prefix flags");
         if (prefix->groups < 0 || prefix->max_len < 0) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "bad prefix groups or max_len");
         if (prefix->groups > 0 && (!prefix->d_off || !prefix->d_len))
             return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "prefix d_off or d_len is NULL");

@@ -72,7 +72,12 @@ Split plan_step(const StepArgs& a, bool work) {
         return (int)std::max<int64_t>(1, ((int64_t)len + chunk - 1) / chunk);
     };
     s.own_parts = parts(units, max_len, 256, 512, s.own_chunk);
-    const bool shares = groups > 0 && max_prefix > 0;
+    // Reading a prefix once costs the joining of its parts and a workgroup's wait for the others. It is worth that where reading
+    // it for every row takes longer: from about 200 MB of keys and values, much of which comes from the caches (us, shared / not, 8
+    // key heads of 128: 16 rows of 2000 15.6 / 14.2, of 8000 20 / 28, 64 of 500 15.6 / 12.5, of 1000 16.3 / 17.3, of 4000 21 / 45,
+    // 128 of 4000 24 / 85; 4 key heads: 64 of 2000 19.1 / 18.7).
+    const bool shares = groups > 0 && max_prefix > 0 &&
+                        ((a.prefix.flags & VXS_FLAG_SHARE_ALWAYS) || (double)rows * max_prefix * kv_heads * a.cache.head_dim * 4 >= 2e8);
     // Short rows, more than fit at once: a wave each, with nothing to join (us, one wave / four: 1024 of (row, key head) with
     // 32 keys 6.3 / 10.8, with 200 18.3 / 21.9, 300 24.6 / 25.6, 500 36.6 / 34.8; 512 with 100 keys 9.6 / 7.4).
     s.solo = units > 512 && max_len - (shares ? max_prefix : 0) <= 256;
@@ -320,18 +325,26 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
                     f4{w.o[d][4 * j], w.o[d][4 * j + 1], w.o[d][4 * j + 2], w.o[d][4 * j + 3]};
     }
     sync();
-    const int w0 = solo ? wv : 0, w1 = solo ? wv + 1 : kWaves;
     float m, l;
     auto joined = [&](int q, int d) {  // entries d..d + 3 of the sums of query row rho0 + q; sets m and l
+        float2 x[kWaves];
+        f4 y[kWaves];
         m = kLowest;
-        for (int i = w0; i < w1; i++) m = fmaxf(m, wave_ml[(i * kCols + q) * 2]);
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) {
+            const int from = solo ? wv : i;
+            x[i] = *reinterpret_cast<const float2*>(wave_ml + (from * kCols + q) * 2);
+            y[i] = *reinterpret_cast<const f4*>(lds + from * kWaveBytes<D> + (q * OS + d) * 4);
+            m = fmaxf(m, x[i].x);
+        }
         f4 o{0.f, 0.f, 0.f, 0.f};
         l = 0.f;
-        for (int i = w0; i < w1; i++) {
-            const float2 x = *reinterpret_cast<const float2*>(wave_ml + (i * kCols + q) * 2);
-            const float f = __builtin_amdgcn_exp2f(x.x - m);
-            l = __builtin_fmaf(x.y, f, l);
-            o = o + *reinterpret_cast<const f4*>(lds + i * kWaveBytes<D> + (q * OS + d) * 4) * f;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) {
+            if (solo && i) break;
+            const float f = __builtin_amdgcn_exp2f(x[i].x - m);
+            l = __builtin_fmaf(x[i].y, f, l);
+            o = o + y[i] * f;
         }
         return o;
     };
