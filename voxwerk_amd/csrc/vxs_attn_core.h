@@ -39,6 +39,7 @@ struct Vec<__bf16> {
     using v8 = bf8;
     static constexpr unsigned kExponent = 0x7F80u;  // all ones: infinity or NaN
     static constexpr float kAbove = 8.0f;           // = kLag: m over the maximum when it is set
+    static constexpr int kParts = 3;                // of an fp32 value: 8 bits each
     static __device__ __forceinline__ f16v mfma(bf8 a, bf8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -47,6 +48,7 @@ struct Vec<_Float16> {
     using v8 = h8;
     static constexpr unsigned kExponent = 0x7C00u;
     static constexpr float kAbove = 0.0f;
+    static constexpr int kParts = 2;  // 11 bits each
     static __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -183,7 +185,7 @@ __device__ __forceinline__ bool scrub(char* rows, int row0, int end, bool each, 
 }
 
 // A wave's 32 queries: operand, running maximum, sum of its own keys' weights, and outputs O^T.
-template <int D, typename T, bool SPLIT>
+template <int D, typename T, int PARTS>
 struct Queries {
     using G = TileGeom<D>;
     using v8 = typename Vec<T>::v8;
@@ -277,30 +279,34 @@ struct Queries {
         const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * t + 8) * G::kRow + ((64 * b) ^ (unit << 4) ^ 32)));
         return s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     }
-    static __device__ __forceinline__ v8 weights(const f16v& s, int t, v8& rest) {
-        v8 hi;
+    // Eight weights in PARTS of T's bits, each the rounded rest of those before.
+    static __device__ __forceinline__ void weights(const f16v& s, int t, v8 (&part)[PARTS]) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            hi[e] = (T)s[8 * t + e];
-            if (SPLIT) rest[e] = (T)(s[8 * t + e] - (float)hi[e]);
+            float rest = s[8 * t + e];
+#pragma unroll
+            for (int i = 0; i < PARTS; i++) {
+                part[i][e] = (T)rest;
+                rest -= (float)part[i][e];
+            }
         }
-        return hi;
     }
 
-    // O^T += V^T P^T over NB x 32 keys. The weights are rounded to T once (SPLIT: the rest of each in a second product). A
-    // weight of zero hides values that are finite only: see scrub().
+    // O^T += V^T P^T over NB x 32 keys. The weights are rounded to T once, as the outputs are: half an ulp of each weight, at random,
+    // is as much of the output as its own rounding. Outputs in fp32 take PARTS products instead, of all the weights' bits that
+    // matter to them. A weight of zero hides values that are finite only: see scrub().
     template <int NB>
     __device__ __forceinline__ void add(const char* tile, const f16v (&s)[NB], int lane) {
-        v8 hi[2 * NB], lo[2 * NB];
+        v8 part[2 * NB][PARTS];
 #pragma unroll
-        for (int k = 0; k < 2 * NB; k++) hi[k] = weights(s[k >> 1], k & 1, lo[k]);
+        for (int k = 0; k < 2 * NB; k++) weights(s[k >> 1], k & 1, part[k]);
 #pragma unroll
         for (int b = 0; b < D / 32; b++)
 #pragma unroll
             for (int k = 0; k < 2 * NB; k++) {
                 const v8 v = __builtin_bit_cast(v8, values(tile, k, b, lane));
-                o[b] = Vec<T>::mfma(v, hi[k], o[b]);
-                if (SPLIT) o[b] = Vec<T>::mfma(v, lo[k], o[b]);
+#pragma unroll
+                for (int i = PARTS - 1; i >= 0; i--) o[b] = Vec<T>::mfma(v, part[k][i], o[b]);
             }
     }
 

@@ -34,7 +34,7 @@ template <int D, typename T, typename TO, int QW, int KW>
 __global__ __launch_bounds__(64 * QW * KW, D == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
     using S = Shape<D, QW, KW>;
     constexpr int TB = S::kTile, NB = S::kKeys / 32, GB = 16 * 2 * D, kRows = S::kRows, kKeys = S::kKeys;
-    constexpr bool SPLIT = sizeof(TO) == 4;
+    constexpr int PARTS = sizeof(TO) == 4 ? Vec<T>::kParts : 1;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wv = wave % QW, kg = wave / QW;
     const int kvh = a.cache.kv_heads, G = a.q_heads / kvh;
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 ? 1 : 2) void attn_prompt_ke
     const int slot = a.slots ? scalar(a.slots, seq) : seq;
     const int len = (int)cache_length(a.cache, slot, scalar(a.kv_len, seq));
 
-    Queries<D, T, SPLIT> w;
+    Queries<D, T, PARTS> w;
     w.init();
     const int col = wv * 32 + (lane & 31);
     const int rho = rho0 + min(col, rows - 1);

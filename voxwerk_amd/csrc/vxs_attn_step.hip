@@ -174,7 +174,7 @@ constexpr int kLdsBytes = kWaves * (kWaveBytes<D> + kCols * 8) + kCols * 4;
 template <int D, typename T, typename TO>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(KernelArgs args) {
     constexpr int KT = kTile<D>, NB = KT / 32, NG = KT / 16, NI = KT * 2 * D / 1024, TB = KT * 2 * D;
-    constexpr bool SPLIT = sizeof(TO) == 4;
+    constexpr int PARTS = sizeof(TO) == 4 ? Vec<T>::kParts : 1;
     constexpr int OS = D + 4;  // floats of a row of the wave's sums
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* wave_ml = reinterpret_cast<float*>(lds + kWaves * kWaveBytes<D>);  // [waves][32][2]
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         fetch(v_base, v_lds);
     }
     const int col = lane & 31;
-    Queries<D, T, SPLIT> w;
+    Queries<D, T, PARTS> w;
     w.init();
     const int rho = rho0 + min(col, cols - 1);
     const int over = pre ? sp.group.div(rho) : 0, row = rbase + over, qh = head * G + rho - over * G;
