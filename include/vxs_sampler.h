@@ -432,7 +432,7 @@ typedef struct vxs_shared_prefix {
  * A few new tokens of one long sequence can be rows too: the same slot, a length each, their context as a shared prefix.
  *
  * work: device memory of vxs_attn_step_workspace bytes, 16-byte aligned, zeroed once before its first use; calls
- * leave it ready for the next. One call at a time may use it (calls on one stream are in order). NULL: each row's keys
+ * leave it ready for the next, of whatever sizes and types. One call at a time may use it (calls on one stream are in order). NULL: each row's keys
  * are read by one workgroup per key head, with no sharing.
  * Asynchronous on the context stream; may be captured.
  */
@@ -441,7 +441,8 @@ VXS_API int vxs_attn_step_device(vxs_ctx* ctx, int rows, int q_heads, const void
                                  const vxs_shared_prefix* prefix, float scale, void* out, int64_t ldo, int out_dtype,
                                  void* work, int64_t work_bytes);
 
-/* The workspace of vxs_attn_step_device calls of at most these sizes, in bytes; negative: an error code. */
+/* The workspace of vxs_attn_step_device calls of at most these rows, max_len and prefix lengths (prefix NULL: calls without
+ * one) over caches of these head sizes, in bytes; negative: an error code. */
 VXS_API int64_t vxs_attn_step_workspace(vxs_ctx* ctx, int rows, int q_heads, const vxs_kv_cache* cache, int max_len,
                                         const vxs_shared_prefix* prefix);
 

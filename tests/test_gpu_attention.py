@@ -172,6 +172,40 @@ def test_step_workspace_is_ready_again(ctx):
             assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
 
 
+def test_step_workspace_serves_other_sizes(ctx):
+    """One workspace, zeroed once, between calls whose rows, parts, head sizes and types differ: each is right."""
+    share = [(0, 24, 500)]
+    # (cache, query heads, prefixes): many parts of few rows come before few parts of many
+    calls = [
+        (Paged([2900, 1500], 2, 128, 16, seed=1), 8, ()),
+        (Paged([700] * 24, 2, 128, 16, seed=2), 8, ()),
+        (Paged([2600], 1, 64, 16, "f16", seed=3), 5, ()),
+        (Paged([700] * 24, 2, 128, 16, seed=4, share=share), 8, share),
+        (Paged([900, 300, 0, 1700, 65], 2, 256, 32, "f16", seed=5), 2, ()),
+        (Paged([600] * 40, 3, 64, 16, seed=6), 12, ()),
+    ]
+    n = max(ctx.attn_step_workspace(len(p.lens), h, p.cache, max(p.lens), SharedPrefix(1, 16, 16, 500, True) if s else None) for p, h, s in calls)
+    work = device(np.zeros(n, np.uint8))
+    for _ in range(2):
+        for i, (p, h, s) in enumerate(calls):
+            step_and_check(ctx, p, h, "f32", share=s, work=work, what=f"call {i}")
+
+
+def test_step_workspace_of_larger_sizes_is_enough(ctx):
+    """A workspace for the largest batch and length serves every smaller call: fewer rows divide their keys further."""
+    paged = Paged([1800] * 24, 2, 128, 16, seed=7)
+    for prefix in (None, SharedPrefix(1, 16, 16, 900, True)):
+        n = ctx.attn_step_workspace(24, 8, paged.cache, 1800, prefix)
+        for rows in range(25):
+            for most in (0, 1, 256, 257, 700, 1800):
+                assert ctx.attn_step_workspace(rows, 8, paged.cache, most, prefix) <= n
+                assert ctx.attn_step_workspace(rows, 8, paged.cache, most) <= n
+    work = device(np.zeros(ctx.attn_step_workspace(24, 8, paged.cache, 1800), np.uint8))
+    for rows in (24, 1, 5, 24, 13):
+        few = Paged([1800] * rows, 2, 128, 16, seed=rows)
+        step_and_check(ctx, few, 8, "f32", work=work, what=f"{rows} rows")
+
+
 def test_step_captured(ctx):
     """A captured step, replayed between other work, gives what an eager one gives."""
     lib = hip.lib()

@@ -53,7 +53,7 @@ struct StepArgs {
     int rows, q_heads, max_len;
     void* work;
 };
-// The bytes of `work` that launch_attn_step asks for at a call's sizes (work itself is not looked at).
+// The bytes of `work` that launch_attn_step asks for at sizes up to a call's (work itself is not looked at).
 int64_t attn_step_work_bytes(const StepArgs& a);
 hipError_t launch_attn_step(const StepArgs& a, int dtype, int out_dtype, hipStream_t stream);
 

@@ -101,22 +101,32 @@ Split plan_step(const StepArgs& a, bool work) {
     return s;
 }
 
-// The workspace: a count of arrived query rows per (row, key head), then the sums: per (row, key head), part and
-// query head, m and l, and D entries of o. A part's sums are written and read at the device's common memory (agent
-// scope: past the caches of one XCD); fences over whole caches would cost more than the step.
+// The workspace: for each (row, key head), part and query head a record of D / 64 blocks of 68 words: m, l, a count, one
+// unused, and 64 entries of o. The count of block i is that of the query rows that have arrived of (row, key head) i; being
+// where no call of any size or type has anything else, counts that a call has set back are zero for the next. A part's sums are
+// written and read at the device's common memory (agent scope: past the caches of one XCD); fences over whole caches would
+// cost more than the step.
+constexpr int kBlock = 68;  // words
 struct Records {
-    unsigned* count;
-    float* o;
-    float* ml;
+    float* base;
     int parts;
 };
-int64_t records_counts(int rows, int kv_heads) { return ((int64_t)rows * kv_heads + 3) / 4 * 4; }
-int64_t records_ml(int rows, int q_heads, int parts) { return ((int64_t)rows * q_heads * parts * 2 + 3) / 4 * 4; }  // (what follows is 16-byte aligned)
+int64_t record_bytes(const StepArgs& a, int64_t row_parts) { return 4 * row_parts * a.q_heads * (a.cache.head_dim / 64) * kBlock; }
 
-int64_t work_bytes(const StepArgs& a, const Split& s) {
-    const int parts = s.own_parts + s.pre_parts;
-    if (parts <= 1) return 0;
-    return 4 * (records_counts(a.rows, a.cache.kv_heads) + records_ml(a.rows, a.q_heads, parts) + (int64_t)a.rows * a.q_heads * parts * a.cache.head_dim);
+// Enough for every call of up to a.rows rows, a.max_len tokens and a.prefix.max_len shared ones (whatever its groups): sums over
+// rows of plan_step's parts, which are at most min(ceil(fill / units), ceil(len / 256), kMaxParts) of a row's keys.
+int64_t work_bytes(const StepArgs& a) {
+    const int64_t rows = a.rows, kv_heads = a.cache.kv_heads, G = a.q_heads / kv_heads, k = kv_heads * ((G + kCols - 1) / kCols);
+    const int64_t most = a.cache.ld_table << a.cache.page_bits, len = std::min<int64_t>(a.max_len, most);
+    auto parts = [](int64_t len, int64_t least) { return std::max<int64_t>(1, std::min<int64_t>((len + least - 1) / least, kMaxParts)); };
+    if (a.prefix.groups == 0) {
+        const int64_t split = std::min(rows, 511 / k);  // more rows than these are not divided
+        return len <= 256 || split == 0 ? 0 : record_bytes(a, std::min(split * parts(len, 256), 512 / k + split));
+    }
+    const int64_t shared = std::min<int64_t>(a.prefix.max_len, most);
+    int64_t own = std::min(rows * parts(len, 256), 512 / k + rows);
+    if (rows * k > 512) own = std::max(own, rows * parts(std::min(len, shared + 256), 1024));
+    return record_bytes(a, own + std::min(rows * parts(shared, 256), 256 * kCols / a.q_heads + rows));
 }
 
 __device__ __forceinline__ void put2(float* p, float a, float b) {
@@ -364,13 +374,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     }
 
     // ---- leave the sums, count the query rows that have arrived
-    auto record = [&](int r, int p, int q) { return (((int64_t)r * sq.heads.d + head) * rec.parts + p) * G + q; };
+    auto record = [&](int r, int p, int q) {
+        return rec.base + ((((int64_t)r * sq.heads.d + head) * rec.parts + p) * G + q) * (D / 64 * kBlock);
+    };
+    auto entries = [](int d) { return d / 64 * kBlock + 4 + d % 64; };
     for (int q = tid / L; q < cols; q += threads / L) {
         const f4 x = joined(q, d4);
         const int up = pre ? sq.group.div(rho0 + q) : 0;
-        const int64_t to = record(rbase + up, pre ? sq.own_parts + part : part, rho0 + q - up * G);
-        put4(rec.o + to * D + d4, x);
-        if (d4 == 0) put2(rec.ml + to * 2, m, l);
+        float* const to = record(rbase + up, pre ? sq.own_parts + part : part, rho0 + q - up * G);
+        put4(to + entries(d4), x);
+        if (d4 == 0) put2(to, m, l);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     sync();
@@ -381,7 +394,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         if (pre) len = (int)cache_length(b.cache, b.slots ? b.slots[r] : r, b.kv_len[r]);
         const int own = parts_of(len - shared, sq.own_chunk, sq.own_parts), pres = parts_of(shared, sq.pre_chunk, sq.pre_parts);
         const unsigned n = pre ? min((first + tid + 1) * G, rho0 + cols) - max((first + tid) * G, rho0) : cols;
-        unsigned* const count = rec.count + (int64_t)r * sq.heads.d + head;
+        unsigned* const count = reinterpret_cast<unsigned*>(rec.base) + ((int64_t)r * sq.heads.d + head) * kBlock + 2;
         const unsigned before = __hip_atomic_fetch_add(count, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const bool done = before + n == (unsigned)((own + pres) * G);
         if (done) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -402,10 +415,10 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
                 ml[u][j] = make_float2(kLowest, 0.f);
                 lo[u][j] = hi[u][j] = make_float2(0.f, 0.f);
                 if (p >= all[u]) continue;
-                const int64_t at = record(row[u], p < own[u] ? p : sq.own_parts + p - own[u], q[u]);
-                ml[u][j] = get2(rec.ml + at * 2);
-                lo[u][j] = get2(rec.o + at * D + 4 * sub);
-                hi[u][j] = get2(rec.o + at * D + 4 * sub + 2);
+                const float* const at = record(row[u], p < own[u] ? p : sq.own_parts + p - own[u], q[u]);
+                ml[u][j] = get2(at);
+                lo[u][j] = get2(at + entries(4 * sub));
+                hi[u][j] = get2(at + entries(4 * sub) + 2);
             }
         };
 #pragma unroll
@@ -453,13 +466,7 @@ template <int D, typename T, typename TO>
 struct Step {
     static hipError_t go(const StepArgs& a, hipStream_t stream) {
         const Split s = plan_step(a, a.work != nullptr);
-        Records r{};
-        r.parts = s.own_parts + s.pre_parts;
-        if (a.work) {
-            r.count = static_cast<unsigned*>(a.work);
-            r.ml = static_cast<float*>(a.work) + records_counts(a.rows, a.cache.kv_heads);
-            r.o = r.ml + records_ml(a.rows, a.q_heads, r.parts);
-        }
+        const Records r{static_cast<float*>(a.work), s.own_parts + s.pre_parts};
         const int64_t own = (int64_t)a.rows * a.cache.kv_heads * s.head_tiles * s.own_parts;
         const int64_t blocks = (int64_t)s.pre_tiles * s.pre_parts * a.cache.kv_heads + (s.solo ? (own + kWaves - 1) / kWaves : own);
         if (blocks > INT32_MAX || own > INT32_MAX) return hipErrorInvalidValue;
@@ -474,7 +481,7 @@ struct Step {
 }  // namespace
 
 int64_t attn_step_work_bytes(const StepArgs& a) {
-    return work_bytes(a, plan_step(a, true));
+    return work_bytes(a);
 }
 
 hipError_t launch_attn_step(const StepArgs& a, int dtype, int out_dtype, hipStream_t stream) {
