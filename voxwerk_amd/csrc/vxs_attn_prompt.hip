@@ -167,9 +167,8 @@ struct Prompt {
         using S = Shape<D, QW, KW>;
         const int64_t tiles = tiles_of(a, S::kRows);
         if (tiles * a.cache.kv_heads > INT32_MAX) return hipErrorInvalidValue;
-        static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW>),
-                                                            hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
-        if (ready != hipSuccess) return ready;
+        static std::atomic<uint64_t> devices{0};
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW>), S::kLds, devices); e != hipSuccess) return e;
         hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,
                            a, (int)tiles);
         return hipGetLastError();

@@ -3,11 +3,23 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/vxs_sampler.h"
 
 namespace vxs {
+
+// Lets a kernel have `bytes` of dynamic LDS on the current device, once for each of them (`devices`: the kernel's own).
+inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& devices) {
+    int d = 0;
+    if (const hipError_t e = hipGetDevice(&d); e != hipSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (d & 63);
+    if (d < 64 && (devices.load(std::memory_order_relaxed) & bit)) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // F<D, T, TO>::go(a, stream) for head_dim D, the cache's type T and the outputs' type TO.
 template <template <int, typename, typename> class F, typename A>
