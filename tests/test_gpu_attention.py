@@ -306,6 +306,35 @@ def test_prompt_nonfinite_after(ctx, dim, dtype):
     assert np.isfinite(late[:, 0][..., ~big]).all() and not np.isfinite(late[:, 0][..., big]).any()
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim,page,dtype,out", [
+    (8, 1, 64, 16, "f16", "f16"), (6, 2, 64, 64, "bf16", "f32"), (4, 2, 128, 16, "bf16", "bf16"), (3, 1, 256, 32, "f16", "f32")])
+def test_prompt_long_contexts(ctx, q_heads, kv_heads, dim, page, dtype, out):
+    """A few new tokens after contexts that end anywhere in the tiles that the waves take in turn."""
+    new, lens = [5, 40, 1, 34, 3, 12, 0, 2], [2500, 2055, 2111, 300, 2, 0, 17, 2304]
+    paged = Paged(lens, kv_heads, dim, page, dtype, seed=dim + q_heads)
+    prompt_and_check(ctx, paged, new, q_heads, out)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (64, "f16"), (128, "f16")])
+def test_prompt_nonfinite_after_long_context(ctx, dim, dtype):
+    """The same behind a long context: earlier new tokens are right, later ones get what they see."""
+    n, new, at = 2200, 90, 2150
+    paged = Paged([n], 2, dim, 16, dtype, seed=dim)
+    p = paged.table[0, at // 16]
+    bad = poison((2, dim), dtype, paged.rng)
+    paged.v[p, :, at % 16] = bad
+    paged.upload()
+    q = rows_of(new, 4, dim, dtype, paged.rng)
+    got = run_prompt(ctx, paged, q, [0, new], 4, dim**-0.5, "f32")
+    first = at - (n - new)  # of the tokens that see it
+    check(got[:first], q[:first], [n - new + j + 1 for j in range(first)], lambda r, h: paged.entries(0, n - new + r + 1, h), 4, 2, dim,
+          dim**-0.5, dtype, "f32", "before")
+    late = got[first:].reshape(new - first, 2, 2, dim)
+    for h in range(2):
+        odd = ~np.isfinite(on.widen(bad[h]))
+        assert np.isfinite(late[:, h][..., ~odd]).all() and not np.isfinite(late[:, h][..., odd]).any()
+
+
 def test_prompt_matches_steps(ctx):
     """The last token of a prompt is a step over the same pages."""
     paged = Paged([90, 200, 33], 2, 128, 16, "bf16", seed=9)

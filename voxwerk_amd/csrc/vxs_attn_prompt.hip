@@ -13,7 +13,7 @@
 // Measured (head_dim 128 unless said): one prompt of 8192, 32 query and 8 key heads, bf16, 533 us: 1.03 PFLOP/s, where a plain product of
 // 8192^3 reaches 1.15; matrix cores busy half of the time at a clock that their load holds near 1.83 GHz, the rest waits on the
 // exponentials of the same wave. 24 prompts of 500 to 1000, 16 and 8 heads: 99 us with bf16 outputs, 154 with fp32 ones, which multiply
-// the values three times. 4 times 65 to 130 tokens after 8000, 32 and 4 heads of 64, fp16: 50 to 55 us, 330 TFLOP/s. One prompt of 93: 8 us.
+// the values three times. 4 times 65 to 130 tokens after 8000, 32 and 4 heads of 64, fp16: 41 to 46 us, 440 TFLOP/s. One prompt of 93: 8 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,7 +36,7 @@ struct Shape {
 };
 
 template <int D, typename T, typename TO, int QW, int KW>
-__global__ __launch_bounds__(64 * QW * KW, D == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
+__global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
     using S = Shape<D, QW, KW>;
     constexpr int TB = S::kTile, NB = S::kKeys / 32, GB = 16 * 2 * D, kRows = S::kRows, kKeys = S::kKeys;
     constexpr int PARTS = sizeof(TO) == 4 ? Vec<T>::kParts : 1;
@@ -183,8 +183,15 @@ struct Prompt {
         // Four groups of two waves (two at D = 256, for the LDS) while 128 rows a workgroup leave compute units idle and a cache
         // may hold more than a few tiles (us, groups / 128 rows: one prompt of 1000 18.8 / 25.5, of 2000, 264 workgroups, 37 / 45,
         // 4 of 500 to 1000, 408 workgroups, 43 / 27; 130 tokens after 8000 91 / 162; one of 93 9.5 / 7.9).
-        if (tiles_of(a, 128) * a.cache.kv_heads <= 288 && (a.cache.ld_table << a.cache.page_bits) > 256)
+        const int64_t keys = a.cache.ld_table << a.cache.page_bits;
+        if (tiles_of(a, 128) * a.cache.kv_heads <= 288 && keys > 256) {
+            // D = 64 leaves LDS for eight groups, one workgroup a compute unit: over long contexts, whose tiles arrive too
+            // late for four (us, eight / four: 4 times 130 after 8000 47 / 56, after 4000 27 / 31, after 2000 18 / 19, one time 64 after
+            // 1000 13.0 / 12.5; 16 times 64 after 2000, 576 workgroups, 31 / 26).
+            if constexpr (D == 64)
+                if (keys > 2048 && tiles_of(a, 64) * a.cache.kv_heads <= 256) return launch<2, 8>(a, stream);
             return launch<2, D == 256 ? 2 : 4>(a, stream);
+        }
         return launch<4, 1>(a, stream);
     }
 };
