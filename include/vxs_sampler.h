@@ -336,7 +336,8 @@ VXS_API int vxs_frame_embed_device(vxs_ctx* ctx, int rows, int groups, int hidde
  * has token_stride = head_dim, head_stride = page_size * head_dim, page_stride = kv_heads * head_stride.
  * A host struct; k, v and table are device memory of the caller's, which also owns the choice of
  * pages (several slots may hold the same page). page_size is a power of two from 16 to 65536, head_dim
- * 64, 128 or 256, the strides are multiples of 8 (token_stride below 2^25, page_stride below 2^31), k and v 16-byte aligned (else VXS_ERR_UNSUPPORTED).
+ * 64, 128 or 256, the strides are multiples of 8 (token_stride below 2^25, page_stride below 2^31), k and v
+ * 16-byte aligned (else VXS_ERR_UNSUPPORTED).
  */
 typedef struct vxs_kv_cache {
     void* k;
@@ -386,7 +387,7 @@ typedef struct vxs_kv_prep {
  *              outside the cache: its key and value are not written
  * Norms, angles and products are fp32 or wider, rounded once, to nearest even. Pointers 16-byte (fp32) or 8-byte
  * (bf16, fp16) aligned, leading dimensions multiples of 4 (q_out: 8-byte, 4), else VXS_ERR_UNSUPPORTED. Two tokens
- * of one call with the same place leave either. Asynchronous on the context stream.
+ * of one call with the same place leave either; tokens is below 2^24. Asynchronous on the context stream.
  */
 VXS_API int vxs_kv_append_device(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, const void* k,
                                  int64_t ldk, const void* v, int64_t ldv, int in_dtype, const vxs_kv_prep* prep,
@@ -432,8 +433,8 @@ typedef struct vxs_shared_prefix {
  * A few new tokens of one long sequence can be rows too: the same slot, a length each, their context as a shared prefix.
  *
  * work: device memory of vxs_attn_step_workspace bytes, 16-byte aligned, zeroed once before its first use; calls
- * leave it ready for the next, of whatever sizes and types. One call at a time may use it (calls on one stream are in order). NULL: each row's keys
- * are read by one workgroup per key head, with no sharing.
+ * leave it ready for the next, of whatever sizes and types. One call at a time may use it (calls on one stream are
+ * in order). NULL: each row's keys are read by one workgroup per key head, with no sharing.
  * Asynchronous on the context stream; may be captured.
  */
 VXS_API int vxs_attn_step_device(vxs_ctx* ctx, int rows, int q_heads, const void* q, int64_t ldq,

@@ -450,3 +450,15 @@ def test_step_shares_where_it_is_faster(ctx, rows, prefix):
     share = [(0, rows, prefix)]
     paged = Paged([prefix + 1 + i % 37 for i in range(rows)], 8, 128, 16, "bf16", seed=rows, share=share)
     step_and_check(ctx, paged, 16, "f32", share=share, always=False)
+
+
+def test_too_many_rows_are_refused(ctx):
+    """A launch's threads are counted in 32 bits: more rows or sequences than that are an error, and nothing is launched."""
+    paged = Paged([40, 20], 2, 64, 16, "bf16", seed=1)
+    x, i32 = device(np.zeros(1 << 14, np.uint16)), device(np.zeros(64, np.int32))
+    with pytest.raises(SamplerError):
+        ctx.attn_step_device(1 << 27, 2, x, 128, paged.cache, i32, 40, 0.1, x, 128, "bf16")
+    with pytest.raises(SamplerError):
+        ctx.attn_prompt_device(1 << 27, 8, 2, x, 128, paged.cache, i32, i32, 0.1, x, 128, "bf16")
+    q = rows_of(2, 2, 64, "bf16", paged.rng)
+    run_step(ctx, paged, q, 2, 0.1)

@@ -184,3 +184,12 @@ def test_refusals(ctx):
         refused(unsupported, **kw)
     call(tokens=0)
     ctx.synchronize()
+
+
+def test_too_many_tokens_are_refused(ctx):
+    """A launch's threads are counted in 32 bits."""
+    paged = Paged([40, 20], 2, 64, 16, "bf16", seed=1)
+    x, i32 = device(np.zeros(1 << 14, np.float32)), device(np.zeros(64, np.int32))
+    with pytest.raises(SamplerError) as e:
+        ctx.kv_append_device(1 << 24, 4, x, 256, None, 0, None, 0, "f32", paged.cache, i32, i32, x, 256)
+    assert e.value.code == _lib.VXS_ERR_UNSUPPORTED and ctx.last_error()

@@ -110,6 +110,7 @@ VXS_API int vxs_kv_append_device(vxs_ctx* ctx, int tokens, int q_heads, const vo
         if ((a.prep.q_norm || a.prep.k_norm) && !(a.prep.eps >= 0.0f))
             return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "eps must not be negative");
         if (a.prep.rot_dim % 8) return ctx_fail(ctx, VXS_ERR_UNSUPPORTED, "rot_dim must be a multiple of 8");
+        if (tokens >= 1 << 24) return ctx_fail(ctx, VXS_ERR_UNSUPPORTED, "tokens must stay below 2^24");
         if (tokens == 0) return vxs::ctx_ok(ctx);
         if (!k != !v) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "k and v come together");
         if (!q && !k) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "neither queries nor keys and values");

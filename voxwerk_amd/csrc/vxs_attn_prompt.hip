@@ -171,7 +171,7 @@ struct Prompt {
     static hipError_t launch(const PromptArgs& a, hipStream_t stream) {
         using S = Shape<D, QW, KW>;
         const int64_t tiles = tiles_of(a, S::kRows);
-        if (tiles * a.cache.kv_heads > INT32_MAX) return hipErrorInvalidValue;
+        if (tiles * a.cache.kv_heads > UINT32_MAX / S::kThreads) return hipErrorInvalidValue;  // (a launch's threads are counted in 32 bits)
         static std::atomic<uint64_t> devices{0};
         if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW>), S::kLds, devices); e != hipSuccess) return e;
         hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,

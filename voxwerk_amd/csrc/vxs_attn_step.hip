@@ -473,7 +473,7 @@ struct Step {
         const Records r{static_cast<float*>(a.work), s.own_parts + s.pre_parts};
         const int64_t own = (int64_t)a.rows * a.cache.kv_heads * s.head_tiles * s.own_parts;
         const int64_t blocks = (int64_t)s.pre_tiles * s.pre_parts * a.cache.kv_heads + (s.solo ? (own + kWaves - 1) / kWaves : own);
-        if (blocks > INT32_MAX || own > INT32_MAX) return hipErrorInvalidValue;
+        if (blocks > UINT32_MAX / kThreads || own > INT32_MAX) return hipErrorInvalidValue;  // (a launch's threads are counted in 32 bits)
         static std::atomic<uint64_t> devices{0};
         if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_step_kernel<D, T, TO>), kLdsBytes<D>, devices); e != hipSuccess) return e;
         hipLaunchKernelGGL((attn_step_kernel<D, T, TO>), dim3((unsigned)blocks), dim3(kThreads), kLdsBytes<D>, stream, KernelArgs{a, s, r});
