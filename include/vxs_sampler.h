@@ -434,7 +434,8 @@ typedef struct vxs_shared_prefix {
  *
  * work: device memory of vxs_attn_step_workspace bytes, 16-byte aligned, zeroed once before its first use; calls
  * leave it ready for the next, of whatever sizes and types. One call at a time may use it (calls on one stream are
- * in order). NULL: each row's keys are read by one workgroup per key head, with no sharing.
+ * in order). Zero it again after a call whose prefix d_off was not ascending or that the device did not finish.
+ * NULL: each row's keys are read by one workgroup per key head, with no sharing.
  * Asynchronous on the context stream; may be captured.
  */
 VXS_API int vxs_attn_step_device(vxs_ctx* ctx, int rows, int q_heads, const void* q, int64_t ldq,
