@@ -1,0 +1,50 @@
+"""GPU checks of attention over a paged cache where sizes change how the work is divided, against the 64-bit oracle."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from voxwerk_amd import hip
+from voxwerk_amd.attention import SharedPrefix
+
+from attention_cases import Paged, as_out, check, device, out_array, rows_of, run_step
+
+pytestmark = pytest.mark.gpu
+
+
+def run_announced(ctx, paged, q, q_heads, scale, out_dtype, kv_len, slots, max_len, off, prefix_len, prefix_max):
+    """A step whose max_len and prefix max_len are capacities, above the real lengths."""
+    rows, width = len(q), q_heads * paged.dim
+    keep = [device(np.array(x, np.int32)) for x in (off, prefix_len, kv_len, slots)]
+    prefix = SharedPrefix(len(prefix_len), keep[0], keep[1], prefix_max, True)
+    n = ctx.attn_step_workspace(rows, q_heads, paged.cache, max_len, prefix)
+    work, dq, out = device(np.zeros(n, np.uint8)), device(q), out_array(rows, width, out_dtype)
+    hip.synchronize()
+    ctx.attn_step_device(rows, q_heads, dq, q.shape[1], paged.cache, keep[2], max_len, scale, out, width, out_dtype, slots=keep[3],
+                         prefix=prefix, workspace=work, workspace_bytes=n)
+    ctx.synchronize()
+    return as_out(out.numpy(), out_dtype)
+
+
+@pytest.mark.parametrize("max_len", [262145, 300000])
+@pytest.mark.parametrize("q_heads,dim,dtype,out", [(1, 64, "bf16", "f32"), (3, 128, "f16", "f16")])
+def test_step_parts_of_a_wave_each(ctx, max_len, q_heads, dim, dtype, out):
+    """More rows than workgroups at once, announced lengths far above the real ones: a long row outside the group is divided
+    among waves that share nothing, at whole granules whatever max_len is."""
+    rows, shared = 514, 48
+    paged = Paged([60, 3500], 1, dim, 16, dtype, seed=dim, width=-(-max_len // 16))
+    kv_len, slots = [60] * (rows - 1) + [3500], [0] * (rows - 1) + [1]
+    q = rows_of(rows, q_heads, dim, dtype, paged.rng, scale=2.0)
+    got = run_announced(ctx, paged, q, q_heads, dim**-0.5, out, kv_len, slots, max_len, [0, rows - 1], [shared], max_len - 100)
+    check(got, q, kv_len, lambda r, h: paged.entries(slots[r], kv_len[r], h), q_heads, 1, dim, dim**-0.5, dtype, out, f"announced {max_len}")
+
+
+@pytest.mark.parametrize("rows,q_heads,kv_heads,dim,dtype,out", [
+    (600, 1, 1, 64, "f16", "f32"), (300, 40, 1, 64, "bf16", "bf16"), (70, 16, 8, 128, "bf16", "f32"), (520, 2, 1, 256, "f16", "f16")])
+def test_step_many_short_rows(ctx, rows, q_heads, kv_heads, dim, dtype, out):
+    """Short rows, more than fit at once, without a prefix: a wave each, lengths around every tile edge, some rows without a key."""
+    lens = [(0, 1, 15, 16, 31, 33, 64, 65, 100, 255, 256)[r % 11] for r in range(rows)]
+    paged = Paged(lens, kv_heads, dim, 16, dtype, seed=rows)
+    q = rows_of(rows, q_heads, dim, dtype, paged.rng, scale=2.0)
+    got = run_step(ctx, paged, q, q_heads, dim**-0.5, out)
+    check(got, q, lens, lambda r, h: paged.entries(r, lens[r], h), q_heads, kv_heads, dim, dim**-0.5, dtype, out, "short rows")
