@@ -1,7 +1,9 @@
-"""Host checks of the paged cache's operators: how a step is divided."""
+"""Host checks of the paged cache's operators: how a step is divided, what their inline assembly holds."""
 from __future__ import annotations
 
+import glob
 import os
+import re
 import subprocess
 
 from voxwerk_amd import build
@@ -15,3 +17,21 @@ def test_step_plans(tmp_path):
                     os.path.join(REPO, "tests", "step_plan.cpp"), "-o", str(exe)], check=True)
     p = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert p.returncode == 0, p.stdout
+
+
+def assembly():
+    """(place, instructions, the rest: operands and what is clobbered) of each inline assembly statement of the attention kernels."""
+    for path in sorted(glob.glob(os.path.join(build.CSRC, "vxs_attn*")) + [os.path.join(build.CSRC, "vxs_append.hip")]):
+        text = open(path, encoding="utf-8").read()
+        for m in re.finditer(r"\basm\b(?:\s+volatile)?\s*\(\s*\"([^\"]*)\"([^;]*);", text):
+            lines = [x.strip() for x in m.group(1).replace("\\t", " ").split("\\n")]
+            yield f"{os.path.basename(path)}:{text.count(chr(10), 0, m.start()) + 1}", [x for x in lines if x], m.group(2)
+
+
+def test_assembly_has_no_vector_arithmetic():
+    """The compiler keeps the wait states between a matrix product (or a vector instruction before a swap of lanes) and the next
+    instruction that reads its result only where it knows that instruction: none of them may be inline assembly."""
+    found = list(assembly())
+    assert len(found) >= 5
+    for place, lines, _ in found:
+        assert not [x for x in lines if x.startswith("v_")], f"{place}: {lines}"

@@ -66,15 +66,13 @@ __device__ __forceinline__ bool any_odd(u4 x) {
     return (y & 0x80008000u) != 0;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {  // (a NaN loses, as in fmaxf, with nothing to canonicalise)
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
+// The largest of three, NaN if one of them is: one instruction. The compiler has to know it, as every one that reads the result of
+// a matrix product: it keeps the wait states between them, and sees no operands in inline assembly.
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 // The larger of a lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return __builtin_elementwise_maximum(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -236,6 +234,7 @@ struct Queries {
             for (int i = 0; i < 16; i += 2) top = max3(top, s[b][i], s[b][i + 1]);
         top = max_halves(top) * c;
         if (__ballot(top > m + (kLag - Vec<T>::kAbove))) {
+            // (where a score is NaN so are the weight and the sums, whatever m is: it stays)
             const float next = fmaxf(m, top + Vec<T>::kAbove), shrink = __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= shrink;
