@@ -35,3 +35,12 @@ def test_assembly_has_no_vector_arithmetic():
     assert len(found) >= 5
     for place, lines, _ in found:
         assert not [x for x in lines if x.startswith("v_")], f"{place}: {lines}"
+
+
+def test_assembly_keeps_what_a_store_reads():
+    """The registers of a store of more than 8 bytes may be written again two wait states after it; the compiler counts none of
+    them for a store that is inline assembly, so they are part of it."""
+    stores = [(place, lines) for place, lines, _ in assembly() if any(re.match(r"global_store_dwordx[34]", x) for x in lines)]
+    assert stores
+    for place, lines in stores:
+        assert re.match(r"global_store_dwordx[34]", lines[-2]) and lines[-1] == "s_nop 1", f"{place}: {lines}"

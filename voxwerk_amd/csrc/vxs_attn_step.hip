@@ -36,8 +36,10 @@ __device__ __forceinline__ void put2(float* p, float a, float b) {
     const uint64_t x = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
     __hip_atomic_store(reinterpret_cast<uint64_t*>(p), x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ void put4(float* p, f4 x) {  // (16-byte aligned; the wait for it is the caller's)
-    asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(x) : "memory");
+// (16-byte aligned; the wait for it is the caller's.) The store reads x's registers after it has been issued: they must keep it for two
+// wait states more, which the compiler does not see.
+__device__ __forceinline__ void put4(float* p, f4 x) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(x) : "memory");
 }
 __device__ __forceinline__ float2 get2(const float* p) {
     const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
