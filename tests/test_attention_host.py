@@ -44,3 +44,16 @@ def test_assembly_keeps_what_a_store_reads():
     assert stores
     for place, lines in stores:
         assert re.match(r"global_store_dwordx[34]", lines[-2]) and lines[-1] == "s_nop 1", f"{place}: {lines}"
+
+
+def test_assembly_of_loads_into_lds():
+    """A load into LDS that is inline assembly names m0, which it overwrites, and holds the five wait states between a vector
+    instruction's writing a scalar register and a load's reading it."""
+    loads = [x for x in assembly() if any(i.startswith("global_load_lds") for i in x[1])]
+    assert loads
+    for place, lines, rest in loads:
+        waits = 0
+        for x in lines[:lines.index(next(i for i in lines if i.startswith("global_load_lds")))]:
+            waits += int(x.split()[1]) + 1 if x.startswith("s_nop") else 1
+        assert lines[0].startswith("s_mov_b32 m0") and waits >= 5, f"{place}: {lines}"
+        assert '"m0"' in rest, f"{place}: {rest}"

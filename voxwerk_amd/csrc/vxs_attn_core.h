@@ -121,15 +121,20 @@ struct Loader {
             off[j] = (unsigned)row * (unsigned)c.token_stride + 16u * (unsigned)((lane % G::kUnits) ^ G::swizzle(row));
         }
     }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is no register that the compiler would save: it only has to know)
     // base: the granule's first row (uniform); lds: where its rows go
     __device__ __forceinline__ void load(const char* base, unsigned lds) const {
         base = uniform_ptr(base);
         lds = uniform((int)lds);
 #pragma unroll
         for (int j = 0; j < G::kLoads; j++)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + 1024u * j), "v"(off[j]), "s"(base)
-                         : "memory");
+            // (inline, or the compiler would wait for all of them before any read of LDS; a base that a vector instruction has just
+            // written needs five wait states before the load, m0 one, and the compiler counts none here)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + 1024u * j), "v"(off[j]), "s"(base)
+                         : "m0", "memory");
     }
+#pragma clang diagnostic pop
 };
 
 // Read-only memory of the launch, read with scalar loads: they are not counted with the loads into LDS.
