@@ -403,8 +403,9 @@ VXS_API int vxs_kv_append_device(vxs_ctx* ctx, int tokens, int q_heads, const vo
  * A token that sees no key gets zeros; keys that a token does not see do not touch its result, whatever they hold.
  * q is of the cache's dtype, out of that or VXS_F32 (leading dimensions in elements, multiples of 8, 16-byte
  * aligned, else VXS_ERR_UNSUPPORTED); scale is positive and finite, q_heads a multiple of kv_heads. Sums and softmax
- * statistics are fp32; the weights are rounded to the cache's type for the matrix cores, and for fp32 outputs
- * kept to 22 bits or more. Rows outside every sequence are not written; a slot outside the cache has no keys, a length above
+ * statistics are fp32. The weights are rounded for the matrix cores: to the cache's type, for fp32 outputs to 24 bits (bf16 caches)
+ * or 22 (fp16). Fp16's range ends this below 2^-21 of a row's largest weight: from there on a weight's error is up to 2^-32 of that
+ * largest one, for fp32 outputs up to 2^-44. bf16's does not end within fp32's. Rows outside every sequence are not written; a slot outside the cache has no keys, a length above
  * the table's is cut to it. Asynchronous on the context stream.
  */
 VXS_API int vxs_attn_prompt_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,

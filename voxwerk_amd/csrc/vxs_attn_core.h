@@ -40,6 +40,7 @@ struct Vec<__bf16> {
     static constexpr unsigned kExponent = 0x7F80u;  // all ones: infinity or NaN
     static constexpr float kAbove = 8.0f;           // = kLag: m over the maximum when it is set
     static constexpr int kParts = 3;                // of an fp32 value: 8 bits each
+    static constexpr float kPart = 1.0f;            // each part is multiplied by this more than the one before
     static __device__ __forceinline__ f16v mfma(bf8 a, bf8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -47,8 +48,9 @@ struct Vec<_Float16> {
     using v4 = h4;
     using v8 = h8;
     static constexpr unsigned kExponent = 0x7C00u;
-    static constexpr float kAbove = 0.0f;
+    static constexpr float kAbove = -7.0f;
     static constexpr int kParts = 2;  // 11 bits each
+    static constexpr float kPart = 2048.0f;
     static __device__ __forceinline__ f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -78,9 +80,8 @@ __device__ __forceinline__ float max_halves(float x) {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.0e38f;  // a running maximum before any key
 // Weights are exp2(score - m), and the sums are rescaled only when some query's maximum has grown by more than kLag since
-// m was set: to the maximum for fp16, whose weights then lie where its precision is and reach 2^kLag (its values end
-// at 2^16, so no sum overflows); for bf16 to kLag above it, so that no weight passes 1 and the type's largest values can be
-// averaged.
+// m was set: for bf16 to kLag above the maximum, so that no weight passes 1; for fp16, whose values end at 2^16 and whose
+// precision ends at 2^-14, to 7 below it: weights reach 2^15, and those down to 2^-21 of the largest keep fp16's bits.
 constexpr float kLag = 8.0f;
 
 template <int N>
@@ -164,6 +165,7 @@ __device__ __forceinline__ uint64_t granule_offset(const PagedCache& c, const in
 // that are not finite, since some query does not see them; true in a lane that found such.
 template <int D, typename T, int BYTES>
 __device__ __forceinline__ bool scrub(char* rows, int row0, int end, bool each, int lane) {
+    asm volatile("" : "+v"(lane));  // (few tiles come here: addresses are formed here too, and hold no registers of the others)
     bool found = false;
 #pragma unroll
     for (int i = 0; i < BYTES / 1024; i++) {
@@ -283,7 +285,8 @@ struct Queries {
         const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (16 * t + 8) * G::kRow + ((64 * b) ^ (unit << 4) ^ 32)));
         return s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     }
-    // Eight weights in PARTS of T's bits, each the rounded rest of those before.
+    // Eight weights in PARTS of T's bits, each the rounded rest of those before, times kPart: an fp16 rest would have nothing left
+    // of its bits for all but the largest weights.
     static __device__ __forceinline__ void weights(const f16v& s, int t, v8 (&part)[PARTS]) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -291,27 +294,44 @@ struct Queries {
 #pragma unroll
             for (int i = 0; i < PARTS; i++) {
                 part[i][e] = (T)rest;
-                rest -= (float)part[i][e];
+                rest = (rest - (float)part[i][e]) * Vec<T>::kPart;
             }
         }
     }
 
     // O^T += V^T P^T over NB x 32 keys. The weights are rounded to T once, as the outputs are: half an ulp of each weight, at random,
-    // is as much of the output as its own rounding. Outputs in fp32 take PARTS products instead, of all the weights' bits that
-    // matter to them. A weight of zero hides values that are finite only: see scrub().
+    // is as much of the output as its own rounding (an fp16 weight below 2^-21 of the largest has an error of 2^-32 of that, so a
+    // million of them stay below the output's rounding). Outputs in fp32 take PARTS products instead, of all the weights' bits that
+    // matter to them: 24 (bf16), or 22, down to 2^-44 of the largest weight (fp16, whose second products have sums of their own until
+    // the end of the tile). A weight of zero hides values that are finite only: see scrub().
     template <int NB>
     __device__ __forceinline__ void add(const char* tile, const f16v (&s)[NB], int lane) {
         v8 part[2 * NB][PARTS];
 #pragma unroll
         for (int k = 0; k < 2 * NB; k++) weights(s[k >> 1], k & 1, part[k]);
 #pragma unroll
-        for (int b = 0; b < D / 32; b++)
+        for (int b = 0; b < D / 32; b++) {
+            if constexpr (PARTS == 1 || Vec<T>::kPart == 1.0f) {
 #pragma unroll
-            for (int k = 0; k < 2 * NB; k++) {
-                const v8 v = __builtin_bit_cast(v8, values(tile, k, b, lane));
+                for (int k = 0; k < 2 * NB; k++) {
+                    const v8 v = __builtin_bit_cast(v8, values(tile, k, b, lane));
 #pragma unroll
-                for (int i = PARTS - 1; i >= 0; i--) o[b] = Vec<T>::mfma(v, part[k][i], o[b]);
+                    for (int i = PARTS - 1; i >= 0; i--) o[b] = Vec<T>::mfma(v, part[k][i], o[b]);
+                }
+            } else {
+                static_assert(PARTS == 2);
+                f16v rest{};
+#pragma unroll
+                for (int k = 0; k < 2 * NB; k++) {
+                    const v8 v = __builtin_bit_cast(v8, values(tile, k, b, lane));
+                    rest = Vec<T>::mfma(v, part[k][1], rest);
+                    o[b] = Vec<T>::mfma(v, part[k][0], o[b]);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] = __builtin_fmaf(rest[i], 1.0f / Vec<T>::kPart, o[b][i]);
+                if (D == 256) __builtin_amdgcn_sched_barrier(0);  // (one block's rest at a time, or registers spill)
             }
+        }
     }
 
     // Adds a key's values that are not finite (row: its values in memory), where this lane's query sees it.
