@@ -114,7 +114,12 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     const int tid = solo ? lane : threadIdx.x, threads = solo ? 64 : kThreads, step = solo ? kTile<D> : kWaves * kTile<D>;
     if (solo) id = id * kWaves + wv;
     auto sync = [&] {
-        if (!solo) __syncthreads();
+        if (!solo) {
+            __syncthreads();
+        } else {  // (a wave's own LDS accesses happen in order; the compiler has to keep it for other lanes' data too)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
     };
     const int rest = sp.heads.div(id);
     head = id - rest * sp.heads.d;
