@@ -28,6 +28,8 @@ void check(const vxs::StepArgs& a, int64_t larger) {
         const vxs::Split s = vxs::plan_step(a, work);
         if (!sound(s.own_parts, s.own_chunk, len)) fail(a, s, "own parts");
         if (s.pre_parts && !sound(s.pre_parts, s.pre_chunk, shared)) fail(a, s, "prefix parts");
+        const int64_t tiles = a.prefix.groups ? (int64_t)a.rows * (a.q_heads / a.cache.kv_heads) / vxs::kCols + a.prefix.groups : 0;
+        if (s.pre_parts && s.pre_tiles != std::min<int64_t>(tiles, INT32_MAX)) fail(a, s, "prefix tiles");
         if (!work && (s.own_parts != 1 || s.pre_parts)) fail(a, s, "divided without a workspace");
         const bool joins = s.own_parts + s.pre_parts > 1;
         const int64_t need = joins ? vxs::record_bytes(a, (int64_t)a.rows * (s.own_parts + s.pre_parts)) : 0;
@@ -57,7 +59,7 @@ int main() {
         a.rows = (int)spread(1, 1 << 14);
         a.max_len = (int)(below(3) ? spread(1, INT32_MAX - 256) : edges[below(sizeof edges / sizeof *edges)]);
         if (below(3)) {
-            a.prefix.groups = (int)spread(1, 300);
+            a.prefix.groups = (int)(i % 64 ? spread(1, 300) : INT32_MAX - below(3));
             a.prefix.flags = below(2) ? VXS_FLAG_SHARE_ALWAYS : 0;
             const int64_t near = a.max_len - below(300);  // (what is left is short: each wave a part of its own)
             a.prefix.max_len = (int)(below(2) ? std::max<int64_t>(near, 1) : spread(1, INT32_MAX - 256));

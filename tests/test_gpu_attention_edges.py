@@ -4,8 +4,9 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from voxwerk_amd import hip
+from voxwerk_amd import _lib, hip
 from voxwerk_amd.attention import SharedPrefix
+from voxwerk_amd.sampler import SamplerError
 
 from attention_cases import Paged, as_out, check, device, out_array, rows_of, run_step
 
@@ -48,3 +49,16 @@ def test_step_many_short_rows(ctx, rows, q_heads, kv_heads, dim, dtype, out):
     q = rows_of(rows, q_heads, dim, dtype, paged.rng, scale=2.0)
     got = run_step(ctx, paged, q, q_heads, dim**-0.5, out)
     check(got, q, lens, lambda r, h: paged.entries(r, lens[r], h), q_heads, kv_heads, dim, dim**-0.5, dtype, out, "short rows")
+
+
+def test_too_many_groups_are_refused(ctx):
+    """More prefix groups than a launch has threads for are an error before anything reads them."""
+    paged = Paged([900, 700], 2, 64, 16, "bf16", seed=1)
+    x, i32 = device(np.zeros(1 << 14, np.uint16)), device(np.zeros(64, np.int32))
+    prefix = SharedPrefix((1 << 31) - 1, i32, i32, 600, True)
+    n = ctx.attn_step_workspace(64, 4, paged.cache, 900, prefix)
+    work = device(np.zeros(n, np.uint8))
+    with pytest.raises(SamplerError):
+        ctx.attn_step_device(64, 4, x, 256, paged.cache, i32, 900, 0.1, x, 256, "bf16", prefix=prefix, workspace=work, workspace_bytes=n)
+    q = rows_of(2, 4, 64, "bf16", paged.rng)
+    run_step(ctx, paged, q, 4, 0.1)

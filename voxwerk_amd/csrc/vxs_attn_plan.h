@@ -74,7 +74,7 @@ inline Split plan_step(const StepArgs& a, bool work) {
         s.own_chunk = INT32_MAX;
     }
     if (shares) {
-        s.pre_tiles = (int)(((int64_t)rows * G) / kCols + groups);
+        s.pre_tiles = (int)std::min<int64_t>(((int64_t)rows * G) / kCols + groups, INT32_MAX);  // (a launch of that many is refused)
         s.pre_parts = parts((int64_t)s.pre_tiles * kv_heads, max_prefix, 256, 256, s.pre_chunk);
     }
     s.group = Divisor::of(G);
