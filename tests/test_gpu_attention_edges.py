@@ -62,3 +62,30 @@ def test_too_many_groups_are_refused(ctx):
         ctx.attn_step_device(64, 4, x, 256, paged.cache, i32, 900, 0.1, x, 256, "bf16", prefix=prefix, workspace=work, workspace_bytes=n)
     q = rows_of(2, 4, 64, "bf16", paged.rng)
     run_step(ctx, paged, q, 4, 0.1)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16"), (256, "bf16")])
+def test_a_workspace_too_small_is_refused(ctx, dim, dtype):
+    """One byte less than vxs_attn_step_workspace says, with and without a prefix, and nothing is written to it."""
+    paged = Paged([1000, 900, 800], 2, dim, 16, dtype, seed=1)
+    rows, q_heads = 3, 4
+    q = rows_of(rows, q_heads, dim, dtype, paged.rng)
+    dq, out, lens = device(q), out_array(rows, q_heads * dim, "f32"), device(np.array(paged.lens, np.int32))
+    prefix = SharedPrefix(1, device(np.array([0, 3], np.int32)), device(np.array([500], np.int32)), 500, True)
+    for p in (None, prefix):
+        n = ctx.attn_step_workspace(rows, q_heads, paged.cache, 1000, p)
+        assert n > 0
+        work = device(np.zeros(n, np.uint8))
+        for short in (n - 1, 16, 0, -1):
+            with pytest.raises(SamplerError) as e:
+                ctx.attn_step_device(rows, q_heads, dq, q_heads * dim, paged.cache, lens, 1000, 0.1, out, q_heads * dim, "f32", prefix=p,
+                                     workspace=work, workspace_bytes=short)
+            assert e.value.code == _lib.VXS_ERR_INVALID_ARG and "vxs_attn_step_workspace" in ctx.last_error()
+        ctx.synchronize()
+        assert not work.numpy().any() and (out.numpy() == 7).all()
+    with_prefix = ctx.attn_step_workspace(rows, q_heads, paged.cache, 1000, prefix)
+    without = ctx.attn_step_workspace(rows, q_heads, paged.cache, 1000)
+    assert without < with_prefix  # (a workspace for calls without a prefix does not serve one with it)
+    with pytest.raises(SamplerError):
+        ctx.attn_step_device(rows, q_heads, dq, q_heads * dim, paged.cache, lens, 1000, 0.1, out, q_heads * dim, "f32", prefix=prefix,
+                             workspace=device(np.zeros(without, np.uint8)), workspace_bytes=without)
