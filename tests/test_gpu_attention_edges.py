@@ -1,14 +1,16 @@
 """GPU checks of attention over a paged cache where sizes change how the work is divided, against the 64-bit oracle."""
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 
 from voxwerk_amd import _lib, hip
 from voxwerk_amd.attention import SharedPrefix
-from voxwerk_amd.sampler import SamplerError
+from voxwerk_amd.sampler import Context, SamplerError
 
-from attention_cases import Paged, as_out, check, device, out_array, rows_of, run_step
+from attention_cases import Paged, as_out, check, device, out_array, rows_of, run_prompt, run_step
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +91,68 @@ def test_a_workspace_too_small_is_refused(ctx, dim, dtype):
     with pytest.raises(SamplerError):
         ctx.attn_step_device(rows, q_heads, dq, q_heads * dim, paged.cache, lens, 1000, 0.1, out, q_heads * dim, "f32", prefix=prefix,
                              workspace=device(np.zeros(without, np.uint8)), workspace_bytes=without)
+
+
+@pytest.mark.parametrize("seqs", [64, 65, 130, 200])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,dtype,out", [(4, 2, 64, "bf16", "f32"), (16, 8, 128, "f16", "f16"), (40, 1, 128, "bf16", "bf16")])
+def test_prompts_of_many_sequences(ctx, seqs, q_heads, kv_heads, dim, dtype, out):
+    """A tile's sequence is looked for among 64 at a time: more of them, empty ones and ones without keys among them."""
+    new = [(3, 0, 1, 40, 0, 9, 33)[i % 7] for i in range(seqs)]
+    lens = [0 if i % 11 == 3 else n + (i * 5) % 23 for i, n in enumerate(new)]
+    paged = Paged(lens, kv_heads, dim, 16, dtype, seed=seqs)
+    off = np.concatenate([[0], np.cumsum(new)])
+    q = rows_of(int(off[-1]), q_heads, dim, dtype, paged.rng, scale=2.0)
+    got = run_prompt(ctx, paged, q, off, q_heads, dim**-0.5, out)
+    whose = np.repeat(np.arange(seqs), new)
+    limits = [max(0, lens[i] - new[i] + j + 1) for i in range(seqs) for j in range(new[i])]
+    check(got, q, limits, lambda r, h: paged.entries(whose[r], limits[r], h), q_heads, kv_heads, dim, dim**-0.5, dtype, out, f"{seqs} prompts")
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,dim,dtype,out", [(4, 2, 64, "f16", "f32"), (16, 1, 128, "bf16", "bf16")])
+def test_step_of_many_groups(ctx, q_heads, kv_heads, dim, dtype, out):
+    """More than 64 groups of different prefixes: of several rows, of one, of none; rows outside every group after them."""
+    share, lens = [], []
+    for g in range(150):
+        rows, prefix = (2, 0, 3, 1, 5)[g % 5], 17 + (g * 13) % 120
+        share.append((len(lens), len(lens) + rows, prefix))
+        lens += [prefix + 1 + (g + i * 7) % 40 for i in range(rows)]
+    lens += [0, 77, 300]
+    paged = Paged(lens, kv_heads, dim, 16, dtype, seed=9, share=share)
+    q = rows_of(len(lens), q_heads, dim, dtype, paged.rng, scale=2.0)
+    got = run_step(ctx, paged, q, q_heads, dim**-0.5, out, share=share)
+    check(got, q, lens, lambda r, h: paged.entries(r, lens[r], h), q_heads, kv_heads, dim, dim**-0.5, dtype, out, "many groups")
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,dim,dtype,out", [(8, 2, 128, "bf16", "f32"), (4, 1, 64, "f16", "f16"), (2, 1, 256, "bf16", "bf16")])
+def test_step_and_prompt_long_rows(ctx, q_heads, kv_heads, dim, dtype, out):
+    lens = [20011, 9000, 1]
+    paged = Paged(lens, kv_heads, dim, 32, dtype, "tokens", seed=5)
+    q = rows_of(3, q_heads, dim, dtype, paged.rng, scale=2.0)
+    for what, got in (("step", run_step(ctx, paged, q, q_heads, dim**-0.5, out)), ("prompt", run_prompt(ctx, paged, q, [0, 1, 2, 3], q_heads, dim**-0.5, out))):
+        check(got, q, lens, lambda r, h: paged.entries(r, lens[r], h), q_heads, kv_heads, dim, dim**-0.5, dtype, out, what)
+
+
+def test_steps_of_two_contexts_at_once(ctx):
+    """Two threads, a context, a stream and a workspace each, over one cache: every step has the bits that it has alone."""
+    share = [(0, 24, 400)]
+    paged = Paged([700 + 11 * i for i in range(24)], 2, 128, 16, "bf16", seed=3, share=share)
+    qs = [rows_of(24, 8, 128, "bf16", paged.rng, scale=2.0) for _ in range(2)]
+    alone = [run_step(ctx, paged, q, 8, 0.1, "f32", share=share) for q in qs]
+    rounds, failed = 20, []
+
+    def work(q, want):
+        try:
+            with Context(0) as own:
+                for i in range(rounds):
+                    got = run_step(own, paged, q, 8, 0.1, "f32", share=share)
+                    if not np.array_equal(got.view(np.uint32), want.view(np.uint32)):
+                        failed.append(i)
+        except Exception as e:  # noqa: BLE001 (reported by the test)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=x) for x in zip(qs, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not failed and not any(t.is_alive() for t in threads), failed
