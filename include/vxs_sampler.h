@@ -387,7 +387,7 @@ typedef struct vxs_kv_prep {
  *              outside the cache: its key and value are not written
  * Norms, angles and products are fp32 or wider, rounded once, to nearest even. Pointers 16-byte (fp32) or 8-byte
  * (bf16, fp16) aligned, leading dimensions multiples of 4 (q_out: 8-byte, 4), else VXS_ERR_UNSUPPORTED. Two tokens
- * of one call with the same place leave either; tokens is below 2^24. Asynchronous on the context stream.
+ * of one call with the same place leave entries of either; tokens is below 2^24. Asynchronous on the context stream.
  */
 VXS_API int vxs_kv_append_device(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, const void* k,
                                  int64_t ldk, const void* v, int64_t ldv, int in_dtype, const vxs_kv_prep* prep,
@@ -400,13 +400,14 @@ VXS_API int vxs_kv_append_device(vxs_ctx* ctx, int tokens, int q_heads, const vo
  * (appended before): its j-th of n new tokens sees the keys up to and with d_kv_len[i] - n + j. For each query head
  * h (key head h / (q_heads / kv_heads)):
  *   out[t][h] = sum_s softmax_s(scale * q[t][h] . k[s]) v[s]
- * A token that sees no key gets zeros; keys that a token does not see do not touch its result, whatever they hold.
+ * A token that sees no key gets zeros; keys that a token does not see do not touch its result, whatever they hold. Where it sees a
+ * value that is infinite or NaN, that entry of its result is infinite or NaN.
  * q is of the cache's dtype, out of that or VXS_F32 (leading dimensions in elements, multiples of 8, 16-byte
  * aligned, else VXS_ERR_UNSUPPORTED); scale is positive and finite, q_heads a multiple of kv_heads. Sums and softmax
  * statistics are fp32. The weights are rounded for the matrix cores: to the cache's type, for fp32 outputs to 24 bits (bf16 caches)
  * or 22 (fp16). Fp16's range ends this below 2^-21 of a row's largest weight: from there on a weight's error is up to 2^-32 of that
- * largest one, for fp32 outputs up to 2^-44. bf16's does not end within fp32's. Rows outside every sequence are not written; a slot outside the cache has no keys, a length above
- * the table's is cut to it. Asynchronous on the context stream.
+ * largest one, for fp32 outputs up to 2^-44. bf16's does not end within fp32's. Rows outside every sequence are not written; a slot outside
+ * the cache has no keys, a length above the table's is cut to it. Asynchronous on the context stream.
  */
 VXS_API int vxs_attn_prompt_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,
                                    const vxs_kv_cache* cache, const int32_t* d_slots, const int32_t* d_q_off,
@@ -429,8 +430,8 @@ typedef struct vxs_shared_prefix {
 /*
  * Attention of one token per sequence: row r's query heads over the first d_kv_len[r] tokens of its slot
  * (d_slots[r]; NULL: slot r), its own among them. Results, types and layouts as vxs_attn_prompt_device; a row of
- * length 0 gets zeros. max_len: no length is longer (the work is divided for it; a longer one costs time, not
- * correctness). prefix: NULL, or the rows' shared prefixes.
+ * length 0 gets zeros. max_len: no length is longer (the work is divided for it, and for the prefix's: longer
+ * or much shorter ones cost time, not correctness). prefix: NULL, or the rows' shared prefixes.
  * A few new tokens of one long sequence can be rows too: the same slot, a length each, their context as a shared prefix.
  *
  * work: device memory of vxs_attn_step_workspace bytes, 16-byte aligned, zeroed once before its first use; calls

@@ -77,7 +77,8 @@ def attend(q, k, v, limit, scale):
 def bound(out, mean, reach, top, limit, dim, dtype, out_dtype):
     """The largest error of an fp32 computation whose weights are rounded to `dtype` (to twice its bits or more for
     fp32 outputs). A score is off by (dim + 2) 2^-24 |q|.|k| from its sum and by |score| 2^-22 in the exponent's argument, an
-    exponential by 2^-20 of itself; a weight's rounding is half an ulp, and for fp16 at least 2^-25 of the largest weight;
+    exponential by 2^-20 of itself; a weight's rounding is half an ulp, and for fp16 at least 2^-25 of the largest weight (the kernels
+    keep more: closed forms hold them to that, this is for entries at random);
     sums of n terms are off by n 2^-24. Numerator and denominator may err in opposite directions."""
     n = np.maximum(np.asarray(limit, np.float64), 0)
     e = (dim + 2) * 2.0**-24 * reach + top * 2.0**-22 + 2.0**-20

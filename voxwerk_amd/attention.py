@@ -65,9 +65,10 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: Optional[str
     magnitude of cosine and sine. For contexts `factor` times longer than the trained `original_length`:
 
     ``"linear"``  every frequency over `factor` (positions squeezed into the trained range);
-    ``"ntk"``     theta raised by factor^(rot_dim / (rot_dim - 2)): the lowest frequency over `factor`, the highest kept;
-    ``"yarn"``    frequencies that turn more than `beta_fast` times over `original_length` kept, those under `beta_slow`
-                  turns over `factor`, a linear ramp over the index between; magnitude 0.1 ln(factor) + 1."""
+    ``"ntk"``     (NTK-aware scaling) theta raised by factor^(rot_dim / (rot_dim - 2)): the lowest frequency over `factor`, the
+                  highest kept;
+    ``"yarn"``    (YaRN, Peng et al. 2023) frequencies that turn more than `beta_fast` times over `original_length` kept, those
+                  under `beta_slow` turns over `factor`, a linear ramp over the index between; magnitude 0.1 ln(factor) + 1."""
     if rot_dim <= 0 or rot_dim % 2:
         raise ValueError("rot_dim must be positive and even")
     if not (theta > 0 and factor > 0):

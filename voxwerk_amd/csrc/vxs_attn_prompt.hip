@@ -10,10 +10,10 @@
 // all of them, the next one while this one is used. Where that leaves compute units idle, KW such groups of waves take a
 // workgroup's tiles in turn, and their sums are joined through LDS at the end.
 //
-// Measured (head_dim 128 unless said): one prompt of 8192, 32 query and 8 key heads, bf16, 533 us: 1.03 PFLOP/s, where a plain product of
-// 8192^3 reaches 1.15; matrix cores busy half of the time at a clock that their load holds near 1.83 GHz, the rest waits on the
-// exponentials of the same wave. 24 prompts of 500 to 1000, 16 and 8 heads: 99 us with bf16 outputs, 154 with fp32 ones, which multiply
-// the values three times (fp16 caches twice, with sums apart: 144 to 150). 4 times 65 to 130 tokens after 8000, 32 and 4 heads of 64, fp16: 41 to 46 us, 440 TFLOP/s. One prompt of 93: 8 us.
+// Measured (head_dim 128 unless said): one prompt of 8192, 32 query and 8 key heads, bf16, 533 to 564 us: 1.03 PFLOP/s, where a plain product of
+// 8192^3 reaches 1.39; matrix cores busy half of the time at a clock that their load holds near 1.83 GHz, the rest waits on the
+// exponentials of the same wave. 24 prompts of 500 to 1000, 16 and 8 heads: 100 us with bf16 outputs (head_dim 64: 60, 256: 271), 156 with fp32 ones, which multiply
+// the values three times (fp16 caches twice, with sums apart: 144 to 150). 4 times 65 to 130 tokens after 8000, 32 and 4 heads of 64, fp16: 40 to 42 us, 440 TFLOP/s. One prompt of 93: 8 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

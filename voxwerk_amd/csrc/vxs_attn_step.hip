@@ -13,7 +13,7 @@
 //
 // Measured (bf16, 8 key heads of 128 unless said): 256 rows of 1500 to 3000 402 us, 2.36 GB at 5.9 TB/s (a copy: 5.2); 24 of 1000 to 2000
 // 32 us, 4.6 TB/s; 4 of 32,500 to 65,000 with 32 query and 4 key heads 82 us, 4.9 TB/s; 96 rows of two prefixes of 4100 and 150 to 300
-// tokens of their own 39 us, 122 MB (each row reading its prefix itself: 1.7 GB); one row of 37 tokens 5.3 us.
+// tokens of their own 39 us, 122 MB (each row reading its prefix itself: 1.7 GB); one row of 37 tokens 5.5 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
