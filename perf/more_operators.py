@@ -193,7 +193,7 @@ def _cache(case, lens, seed, shared=()):
         if rest and hi - lo > 1:  # (whole blocks: the last of the prefix holds the rows' next tokens too, the same for all)
             for x in (k, v, ks, vs):
                 bits = x.view(torch.uint8)
-                bits[table[lo + 1:hi, whole].long()] = bits[table[lo, whole].long()]
+                bits[table[lo + 1:hi, whole].long()] = bits[table[lo, whole].long()].clone()
     return {"k": k, "v": v, "k_scale": ks, "v_scale": vs, "table": table, "pages": pages, "width": width}
 
 
