@@ -450,6 +450,97 @@ VXS_API int vxs_attn_step_device(vxs_ctx* ctx, int rows, int q_heads, const void
 VXS_API int64_t vxs_attn_step_workspace(vxs_ctx* ctx, int rows, int q_heads, const vxs_kv_cache* cache, int max_len,
                                         const vxs_shared_prefix* prefix);
 
+/*
+ * Cross attention of packed tokens to another sequence's states (an encoder's): as vxs_attn_prompt_device, but every token
+ * [d_q_off[i], d_q_off[i + 1]) sees all d_kv_len[i] tokens of its slot, of which it is none. Both lengths are of any size. One
+ * token per sequence, or a few over many states, are a step's rows too: vxs_attn_step_device's see their whole slot.
+ */
+VXS_API int vxs_attn_cross_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,
+                                  const vxs_kv_cache* cache, const int32_t* d_slots, const int32_t* d_q_off,
+                                  const int32_t* d_kv_len, float scale, void* out, int64_t ldo, int out_dtype);
+
+/*
+ * Positions of several axes for the rotation of queries and keys (time, height and width of images and video between text):
+ * frequency i of vxs_kv_prep turns by the token's position on axis d_axis[i], which is d_pos[d_axis[i] * ld_pos + token].
+ * d_axis int32 [rot_dim / 2] in device memory, 16-byte aligned, entries in [0, axes) (one outside counts as the nearest inside);
+ * ld_pos at least the call's tokens.
+ */
+typedef struct vxs_rope_axes {
+    const int32_t* d_axis;
+    int64_t ld_pos;
+    int32_t axes;
+} vxs_rope_axes;
+
+/* vxs_kv_append_device with d_pos int32 [axes][ld_pos]; d_index, each token's place in its sequence, is needed with k and v.
+ * axes NULL: vxs_kv_append_device. */
+VXS_API int vxs_kv_append_axes_device(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, const void* k,
+                                      int64_t ldk, const void* v, int64_t ldv, int in_dtype, const vxs_kv_prep* prep,
+                                      const vxs_rope_axes* axes, const int32_t* d_pos, const int32_t* d_slots,
+                                      const int32_t* d_index, const vxs_kv_cache* cache, void* q_out, int64_t ldqo,
+                                      int32_t* d_status);
+
+/*
+ * One layer's cache in 8 bits: as vxs_kv_cache with entries of one byte (OCP e4m3: 4 significant bits, up to 448 in size) and a
+ * scale for each block of 16 tokens and key head, for keys and values apart. Block b of a slot is its tokens 16 b .. 16 b + 15;
+ * its scale of head h is the byte (page * kv_heads + h) * (page_size / 16) + (16 b % page_size) / 16 of k_scale, which stands for
+ * 2^(byte - 127) (E8M0; 1 to 254), and its entries for e4m3 * 2^(byte - 127). Strides in entries, multiples of 16, k and v
+ * 16-byte aligned; k_scale and v_scale 4-byte aligned and read in whole 4-byte words (else VXS_ERR_UNSUPPORTED).
+ * q_dtype: the type of queries, VXS_BF16 or VXS_F16.
+ */
+typedef struct vxs_kv8_cache {
+    void* k;
+    void* v;
+    uint8_t* k_scale; /* [pages][kv_heads][page_size / 16] */
+    uint8_t* v_scale;
+    const int32_t* table;
+    int64_t ld_table;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t token_stride;
+    int32_t slots;
+    int32_t pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t q_dtype;
+} vxs_kv8_cache;
+
+/*
+ * vxs_kv_append_device and vxs_kv_append_axes_device (axes NULL: one position a token) for an 8-bit cache; queries go to q_out in
+ * q_dtype. A block's scale is the least power of two (from 2^-126) with which none of its finite entries, as they are in fp32
+ * after norm and rotation, passes 448; entries are divided by it and rounded once, to nearest even, infinite ones and NaN
+ * become NaN. A token at the first place of a block begins it anew: what the block held counts for nothing. Tokens at other
+ * places join what is there: where they need a larger scale, the entries at the block's other places are divided by the
+ * quotient, a power of two, which changes none but those that fall below 2^-6 of the new scale (rounded to its 2^-9).
+ * Tokens of one block in one call are consecutive rows (of two with the same place the later one stays); where they are not,
+ * what that block holds after the call is unspecified, as where two slots that share its page append to it.
+ */
+VXS_API int vxs_kv8_append_device(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, const void* k,
+                                  int64_t ldk, const void* v, int64_t ldv, int in_dtype, const vxs_kv_prep* prep,
+                                  const vxs_rope_axes* axes, const int32_t* d_pos, const int32_t* d_slots,
+                                  const int32_t* d_index, const vxs_kv8_cache* cache, void* q_out, int64_t ldqo,
+                                  int32_t* d_status);
+
+/*
+ * vxs_attn_prompt_device, vxs_attn_cross_device, vxs_attn_step_device and vxs_attn_step_workspace over an 8-bit cache: the same
+ * but for the cache; q is of its q_dtype, out of that or VXS_F32. Keys and values enter the products as they are (e4m3 has fewer
+ * bits than bf16 and fp16), values times their scale; the weights are rounded to 8 significant bits for bf16 outputs, 16 for fp16,
+ * 24 for fp32; sums are fp32, whose range ends: outputs may be off by 2^-116 whatever the scales. A NaN entry that a token sees
+ * makes its result NaN (a key's: all of it, a value's: that entry). A workspace serves steps over both kinds of cache.
+ */
+VXS_API int vxs_attn8_prompt_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,
+                                    const vxs_kv8_cache* cache, const int32_t* d_slots, const int32_t* d_q_off,
+                                    const int32_t* d_kv_len, float scale, void* out, int64_t ldo, int out_dtype);
+VXS_API int vxs_attn8_cross_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,
+                                   const vxs_kv8_cache* cache, const int32_t* d_slots, const int32_t* d_q_off,
+                                   const int32_t* d_kv_len, float scale, void* out, int64_t ldo, int out_dtype);
+VXS_API int vxs_attn8_step_device(vxs_ctx* ctx, int rows, int q_heads, const void* q, int64_t ldq,
+                                  const vxs_kv8_cache* cache, const int32_t* d_slots, const int32_t* d_kv_len, int max_len,
+                                  const vxs_shared_prefix* prefix, float scale, void* out, int64_t ldo, int out_dtype,
+                                  void* work, int64_t work_bytes);
+VXS_API int64_t vxs_attn8_step_workspace(vxs_ctx* ctx, int rows, int q_heads, const vxs_kv8_cache* cache, int max_len,
+                                         const vxs_shared_prefix* prefix);
+
 #ifdef __cplusplus
 }
 #endif

@@ -96,6 +96,21 @@ class VxsKvPrep(ctypes.Structure):
                 ("rope_scale", c_float), ("rot_dim", c_int32), ("interleaved", c_int32)]
 
 
+class VxsKv8Cache(ctypes.Structure):
+    """vxs_kv8_cache (include/vxs_sampler.h)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("table", c_void_p),
+                ("ld_table", c_int64), ("page_stride", c_int64), ("head_stride", c_int64), ("token_stride", c_int64),
+                ("slots", c_int32), ("pages", c_int32), ("page_size", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("q_dtype", c_int32)]
+
+
+class VxsRopeAxes(ctypes.Structure):
+    """vxs_rope_axes (include/vxs_sampler.h)."""
+
+    _fields_ = [("d_axis", c_void_p), ("ld_pos", c_int64), ("axes", c_int32)]
+
+
 class VxsSharedPrefix(ctypes.Structure):
     """vxs_shared_prefix (include/vxs_sampler.h)."""
 
@@ -103,6 +118,10 @@ class VxsSharedPrefix(ctypes.Structure):
 
 
 _P = c_void_p  # raw pointers are passed as integers / c_void_p
+
+_APPEND_AXES = [c_void_p, c_int, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P, _P, _P, _P, _P, _P, c_int64, _P]
+_ATTN_PACKED = [c_void_p, c_int, c_int, c_int, _P, c_int64, _P, _P, _P, _P, c_float, _P, c_int64, c_int]
+_ATTN_STEP = [c_void_p, c_int, c_int, _P, c_int64, _P, _P, _P, c_int, _P, c_float, _P, c_int64, c_int, _P, c_int64]
 
 _SIGNATURES = {
     "vxs_create": (c_int, [POINTER(c_void_p), c_int, c_int, c_int, c_int64]),
@@ -133,11 +152,16 @@ _SIGNATURES = {
                                        c_int64, _P, c_int64, _P]),
     "vxs_kv_append_device": (c_int, [c_void_p, c_int, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P, _P, _P,
                                      _P, _P, c_int64, _P]),
-    "vxs_attn_prompt_device": (c_int, [c_void_p, c_int, c_int, c_int, _P, c_int64, _P, _P, _P, _P, c_float, _P, c_int64,
-                                       c_int]),
-    "vxs_attn_step_device": (c_int, [c_void_p, c_int, c_int, _P, c_int64, _P, _P, _P, c_int, _P, c_float, _P, c_int64,
-                                     c_int, _P, c_int64]),
+    "vxs_kv_append_axes_device": (c_int, _APPEND_AXES),
+    "vxs_kv8_append_device": (c_int, _APPEND_AXES),
+    "vxs_attn_prompt_device": (c_int, _ATTN_PACKED),
+    "vxs_attn_cross_device": (c_int, _ATTN_PACKED),
+    "vxs_attn_step_device": (c_int, _ATTN_STEP),
     "vxs_attn_step_workspace": (c_int64, [c_void_p, c_int, c_int, _P, c_int, _P]),
+    "vxs_attn8_prompt_device": (c_int, _ATTN_PACKED),
+    "vxs_attn8_cross_device": (c_int, _ATTN_PACKED),
+    "vxs_attn8_step_device": (c_int, _ATTN_STEP),
+    "vxs_attn8_step_workspace": (c_int64, [c_void_p, c_int, c_int, _P, c_int, _P]),
     "vxs_history_draw": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, _P]),
     "vxs_sample_batch": (c_int, [c_void_p, c_void_p, c_int, c_int, _P, c_int64, _P, c_int, _P, c_int, _P, _P,
                                  c_uint32]),

@@ -1,8 +1,9 @@
 """Host side of the paged cache and the attention that reads it (include/vxs_sampler.h: vxs_kv_cache and after).
 
-``KvCache``, ``KvPrep`` and ``SharedPrefix`` describe device memory of the caller's (torch tensors, ``hip.DeviceArray``
-or addresses) and keep it alive; ``Context.kv_append_device``, ``attn_prompt_device`` and ``attn_step_device`` take
-them. ``rope_frequencies`` gives the rotation's frequencies for long contexts too.
+``KvCache``, ``Kv8Cache`` (in 8 bits), ``KvPrep``, ``RopeAxes`` and ``SharedPrefix`` describe device memory of the caller's (torch
+tensors, ``hip.DeviceArray`` or addresses) and keep it alive; ``Context.kv_append_device``, ``attn_prompt_device``,
+``attn_cross_device`` and ``attn_step_device`` take them, with either kind of cache. ``rope_frequencies`` gives the rotation's
+frequencies for long contexts too, ``rope_axes`` their axes for images and video.
 """
 from __future__ import annotations
 
@@ -23,6 +24,8 @@ class KvCache:
     ("bf16" or "f16"), as [pages, kv_heads, page_size, head_dim] or with the given strides in entries; `table`: int32
     [slots, ld_table] page numbers."""
 
+    bits = 16
+
     def __init__(self, k, v, dtype: str, kv_heads: int, head_dim: int, pages: int, page_size: int, table, slots: int,
                  ld_table: int, page_stride: Optional[int] = None, head_stride: Optional[int] = None,
                  token_stride: Optional[int] = None):
@@ -33,6 +36,37 @@ class KvCache:
         self.dtype, self.kv_heads, self.head_dim, self.page_size, self.slots = dtype, kv_heads, head_dim, page_size, slots
         self.struct = _lib.VxsKvCache(ptr(k), ptr(v), ptr(table), ld_table, page, head, token, slots, pages, page_size,
                                       kv_heads, head_dim, DTYPES[dtype])
+        self.ref = ctypes.byref(self.struct)
+
+
+class Kv8Cache:
+    """One layer's cache in 8 bits (vxs_kv8_cache). `k`, `v`: one byte (e4m3) an entry, as [pages, kv_heads, page_size, head_dim]
+    or with the given strides in entries; `k_scale`, `v_scale`: bytes (E8M0: b stands for 2^(b - 127)) [pages, kv_heads,
+    page_size / 16], of each 16 tokens; `q_dtype`: the type of queries ("bf16" or "f16"); `table`: int32 [slots, ld_table] page
+    numbers. Takes a KvCache's place in every call."""
+
+    bits = 8
+
+    def __init__(self, k, v, k_scale, v_scale, q_dtype: str, kv_heads: int, head_dim: int, pages: int, page_size: int, table,
+                 slots: int, ld_table: int, page_stride: Optional[int] = None, head_stride: Optional[int] = None,
+                 token_stride: Optional[int] = None):
+        self._keep = (k, v, k_scale, v_scale, table)
+        token = head_dim if token_stride is None else token_stride
+        head = page_size * head_dim if head_stride is None else head_stride
+        page = kv_heads * page_size * head_dim if page_stride is None else page_stride
+        self.dtype, self.kv_heads, self.head_dim, self.page_size, self.slots = q_dtype, kv_heads, head_dim, page_size, slots
+        self.struct = _lib.VxsKv8Cache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), ptr(table), ld_table, page, head, token, slots,
+                                       pages, page_size, kv_heads, head_dim, DTYPES[q_dtype])
+        self.ref = ctypes.byref(self.struct)
+
+
+class RopeAxes:
+    """Positions of several axes (vxs_rope_axes): frequency i turns by the position on axis `axis`[i] (int32 [rot_dim / 2] in
+    device memory; ``rope_axes`` makes the numbers); a call's positions are int32 [axes, ld_pos]."""
+
+    def __init__(self, axis, axes: int, ld_pos: int):
+        self._keep = axis
+        self.struct = _lib.VxsRopeAxes(ptr(axis), ld_pos, axes)
         self.ref = ctypes.byref(self.struct)
 
 
@@ -57,6 +91,24 @@ class SharedPrefix:
         self._keep = (off, length)
         self.struct = _lib.VxsSharedPrefix(ptr(off), ptr(length), groups, max_len, _lib.VXS_FLAG_SHARE_ALWAYS if always else 0)
         self.ref = ctypes.byref(self.struct)
+
+
+def rope_axes(sections, interleaved: bool = False) -> np.ndarray:
+    """The axis of each frequency, int32 [sum(sections)], where axis a has sections[a] of them (time, height, width, say):
+    one section after the other, or interleaved: axis a > 0 has a, a + n, a + 2n, ... of n axes until its section is used up,
+    axis 0 the rest."""
+    n, total = len(sections), sum(sections)
+    if n == 0 or min(sections) < 0 or total == 0:
+        raise ValueError("sections must not be negative, and not all empty")
+    if not interleaved:
+        return np.repeat(np.arange(n, dtype=np.int32), sections)
+    axis = np.zeros(total, np.int32)
+    for a in range(1, n):
+        at = a + n * np.arange(sections[a])
+        if len(at) and at[-1] >= total:
+            raise ValueError(f"section {a} is too long to be interleaved")
+        axis[at] = a
+    return axis
 
 
 def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,

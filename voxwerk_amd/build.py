@@ -32,7 +32,7 @@ HIP_FLAGS = [
     f"-I{INCLUDE}",
 ]
 HIP_SOURCES = ["vxs_kernels.hip", "vxs_wide.hip", "vxs_history.hip", "vxs_embed.hip", "vxs_head.hip", "vxs_noalloc.hip",
-               "vxs_append.hip", "vxs_attn_prompt.hip", "vxs_attn_step.hip", "vxs_attn_api.cpp", "vxs_api.cpp"]
+               "vxs_append.hip", "vxs_append8.hip", "vxs_attn_prompt.hip", "vxs_attn_step.hip", "vxs_attn_api.cpp", "vxs_api.cpp"]
 # Per-source flags. The sampling kernels are scheduled by LLVM's max-ILP strategy with relaxed
 # occupancy targets (same registers, no spills; measured on the same GPU against the default
 # scheduler: headline 4096 x 3072 21.10 -> 20.75 us, batched talker 256 x 3072 12.0-12.3 -> 11.54 us
@@ -71,7 +71,7 @@ def build_hip() -> str:
             src = HIP_SOURCES[i]
             _run([HIPCC, *HIP_FLAGS, *SOURCE_FLAGS.get(src, []), "-c", "-o", objs[i], os.path.join(CSRC, src)])
 
-        with ThreadPoolExecutor(max_workers=min(4, os.cpu_count() or 1)) as ex:
+        with ThreadPoolExecutor(max_workers=min(6, os.cpu_count() or 1)) as ex:
             list(ex.map(compile_one, range(len(HIP_SOURCES))))
         _run([HIPCC, *HIP_FLAGS, "-shared", "-o", tmp, *objs])
     os.replace(tmp, out)

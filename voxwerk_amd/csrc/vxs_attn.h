@@ -8,10 +8,11 @@
 
 namespace vxs {
 
-// A layer's cache as the kernels take it (vxs_kv_cache, checked).
+// A layer's cache as the kernels take it (vxs_kv_cache or vxs_kv8_cache, checked).
 struct PagedCache {
     char* k;
     char* v;
+    uint8_t *k_scale, *v_scale;  // of 8-bit entries, else null
     const int32_t* table;
     int64_t ld_table;
     int64_t head_stride;                 // bytes
@@ -22,6 +23,7 @@ struct PagedCache {
 struct AppendArgs {
     PagedCache cache;
     vxs_kv_prep prep;
+    vxs_rope_axes axes;  // axes 0: one position a token
     const void *q, *k, *v;  // q, or k and v, may be null
     int64_t ldq, ldk, ldv, ldqo;
     const int32_t *pos, *slots, *index;
@@ -30,6 +32,7 @@ struct AppendArgs {
     int tokens, q_heads;
 };
 hipError_t launch_kv_append(const AppendArgs& a, int in_dtype, int dtype, hipStream_t stream);
+hipError_t launch_kv8_append(const AppendArgs& a, int in_dtype, int q_dtype, hipStream_t stream);
 
 struct PromptArgs {
     PagedCache cache;
@@ -39,7 +42,9 @@ struct PromptArgs {
     int64_t ldq, ldo;  // elements
     float scale;
     int seqs, tokens, q_heads;
+    int cross;  // every token sees all of its sequence's keys
 };
+// (dtype: the queries' type; 8-bit entries where the cache has scales)
 hipError_t launch_attn_prompt(const PromptArgs& a, int dtype, int out_dtype, hipStream_t stream);
 
 struct StepArgs {
@@ -70,6 +75,14 @@ __device__ __forceinline__ int64_t cache_length(const PagedCache& c, int slot, i
 __device__ __forceinline__ uint64_t cache_offset(const PagedCache& c, int page, int h, int t) {
     return (uint64_t)min((unsigned)page, (unsigned)c.pages - 1u) * c.page_stride + (uint64_t)h * c.head_stride +
            (uint64_t)((unsigned)t & ((1u << c.page_bits) - 1u)) * c.token_stride;
+}
+
+constexpr int kBlockTokens = 16;  // of an 8-bit cache's scale
+
+// Index of the scale of token t's block of head h, in a page as above.
+__device__ __forceinline__ uint64_t scale_index(const PagedCache& c, int page, int h, int t) {
+    return (((uint64_t)min((unsigned)page, (unsigned)c.pages - 1u) * (unsigned)c.kv_heads + (unsigned)h) << (c.page_bits - 4)) +
+           (((unsigned)t & ((1u << c.page_bits) - 1u)) >> 4);
 }
 #endif
 

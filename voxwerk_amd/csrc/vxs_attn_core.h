@@ -111,9 +111,8 @@ struct TileGeom {
 };
 
 // Loads of 16 rows (a granule: always within one page) of a cache into LDS.
-template <int D>
+template <int D, typename G = TileGeom<D>>
 struct Loader {
-    using G = TileGeom<D>;
     unsigned off[G::kLoads];  // this lane's byte offsets within a granule
     __device__ __forceinline__ void init(const PagedCache& c, int lane) {
 #pragma unroll
@@ -154,10 +153,11 @@ __device__ __forceinline__ A arguments_again() {
 #endif
 }
 
-// Byte offset, from k or v at `head`, of the granule that begins at token t (uniform) of a slot whose table entries are
-// `pages`, the last of them at `last`. Granules past a sequence's end read what is there in the pool.
+// The page of the granule that begins at token t (uniform) of a slot whose table entries are `pages`, the last of them at
+// `last`, and its byte offset from k or v at `head`. Granules past a sequence's end read what is there in the pool.
+__device__ __forceinline__ int granule_page(const PagedCache& c, const int32_t* pages, int last, int t) { return scalar(pages, min(t >> c.page_bits, last)); }
 __device__ __forceinline__ uint64_t granule_offset(const PagedCache& c, const int32_t* pages, int last, int t) {
-    return cache_offset(c, scalar(pages, min(t >> c.page_bits, last)), 0, t);
+    return cache_offset(c, granule_page(c, pages, last, t), 0, t);
 }
 
 // BYTES of a tile of values in LDS (whole rows, the first of which is key `row0` of the tile) before weights of zero meet

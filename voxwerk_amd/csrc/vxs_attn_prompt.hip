@@ -18,28 +18,29 @@
 
 #include <algorithm>
 
-#include "vxs_attn_core.h"
+#include "vxs_attn_core8.h"
 #include "vxs_attn_types.h"
 
 namespace vxs {
 namespace {
 
-template <int D, int QW, int KW>
+template <int D, int QW, int KW, bool E8>
 struct Shape {
     static constexpr int kThreads = 64 * QW * KW;
     static constexpr int kRows = 32 * QW;    // query rows of a workgroup
     static constexpr int kKeys = 16 * QW;    // of a tile: each wave loads a granule of 16
-    static constexpr int kTile = kKeys * 2 * D;
+    static constexpr int kTile = kKeys * (E8 ? D : 2 * D);
     static constexpr int kTiles = KW * 4 * kTile;                             // [groups][2 buffers][keys, values]
     static constexpr int kSums = KW == 1 ? 0 : QW * KW * 32 * (D + 4 + 2) * 4;  // [waves][32][D + 4], [waves][32] m and l
     static constexpr int kLds = kTiles > kSums ? kTiles : kSums;
 };
 
-template <int D, typename T, typename TO, int QW, int KW>
+// T: the queries' type, E8: over 8-bit entries (else of T).
+template <int D, typename T, typename TO, int QW, int KW, bool E8>
 __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
-    using S = Shape<D, QW, KW>;
-    constexpr int TB = S::kTile, NB = S::kKeys / 32, GB = 16 * 2 * D, kRows = S::kRows, kKeys = S::kKeys;
-    constexpr int PARTS = sizeof(TO) == 4 ? Vec<T>::kParts : 1;
+    using S = Shape<D, QW, KW, E8>;
+    constexpr int TB = S::kTile, NB = S::kKeys / 32, NG = S::kKeys / 16, GB = TB / NG, kRows = S::kRows, kKeys = S::kKeys;
+    constexpr int PARTS = weight_parts<T, TO, E8>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wv = wave % QW, kg = wave / QW;
     const int kvh = a.cache.kv_heads, G = a.q_heads / kvh;
@@ -65,30 +66,36 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
     const int slot = a.slots ? scalar(a.slots, seq) : seq;
     const int len = (int)cache_length(a.cache, slot, scalar(a.kv_len, seq));
 
-    Queries<D, T, PARTS> w;
+    std::conditional_t<E8, Queries8<D, T, PARTS>, Queries<D, T, PARTS>> w;
     w.init();
     const int col = wv * 32 + (lane & 31);
     const int rho = rho0 + min(col, rows - 1);
     const int j = rho / G, qh = head * G + rho % G;
-    const int seen = max(len - n + j + 1, 0);
-    const int first = uniform(max(len - n + (rho0 + min(wv * 32, rows - 1)) / G + 1, 0));  // seen by the wave's first row
-    const int last = uniform(max(len - n + (rho0 + min(wv * 32 + 31, rows - 1)) / G + 1, 0));
-    const int all = uniform(max(len - n + rho0 / G + 1, 0));               // keys that every row of the workgroup sees
-    const int end = uniform(max(len - n + (rho0 + rows - 1) / G + 1, 0));  // that some row sees
+    auto limit = [&](int j) { return a.cross ? len : max(len - n + j + 1, 0); };  // keys that token j sees
+    const int seen = limit(j);
+    const int first = uniform(limit((rho0 + min(wv * 32, rows - 1)) / G));  // seen by the wave's first row
+    const int last = uniform(limit((rho0 + min(wv * 32 + 31, rows - 1)) / G));
+    const int all = uniform(limit(rho0 / G));               // keys that every row of the workgroup sees
+    const int end = uniform(limit((rho0 + rows - 1) / G));  // that some row sees
     const float c = a.scale * kLog2e;
 
-    Loader<D> loader;
+    Loader<D, std::conditional_t<E8, TileGeom8<D>, TileGeom<D>>> loader;
     loader.init(a.cache, lane);
     const int32_t* pages = a.cache.table + (int64_t)(end ? slot : 0) * a.cache.ld_table;
     const int last_page = (int)a.cache.ld_table - 1;
     const char* const k_base = a.cache.k + (uint64_t)head * a.cache.head_stride;
     const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
     char* const own = lds + kg * 4 * TB;
+    Scales<E8 ? NG : 1> scales;  // of the tile that was last fetched
     auto fetch = [&](int t, int buffer) {  // each wave 16 of the tile's rows
         const uint64_t at = granule_offset(a.cache, pages, last_page, t + 16 * wv);
         const unsigned to = lds_address(own + buffer * 2 * TB + wv * GB);
         loader.load(k_base + at, to);
         loader.load(v_base + at, to + TB);
+        if constexpr (E8)
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+                scales.read(a.cache, g, granule_page(a.cache, pages, last_page, t + 16 * g), head, t + 16 * g, end);
     };
     if (kg * kKeys < end) fetch(kg * kKeys, 0);
     w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
@@ -99,19 +106,33 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
         const int t = base + kg * kKeys;
         wait_vm<0>();
         __syncthreads();  // the tiles are there, and nobody reads the other buffers any more
+        const Scales<E8 ? NG : 1> now = scales;
         if (t + KW * kKeys < end) fetch(t + KW * kKeys, buffer ^ 1);
         char* const kt = own + buffer * 2 * TB;
         if (base + KW * kKeys > all) {  // some row does not see all of the tiles: each wave looks through its part of the values
-            if (t < end) odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
+            if (t < end) {
+                if constexpr (E8) odd |= scrub8<D, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
+                else odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
+            }
             __syncthreads();
         }
         if (t >= last) continue;
         f16v s[NB];
 #pragma unroll
-        for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 32 * 2 * D, lane);
+        for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 2 * GB, lane);
         if (t + kKeys > first) w.hide(s, seen - t, lane);
-        w.weigh(s, c);
-        w.add(kt + TB, s, lane);
+        if constexpr (E8) {
+            float f[NG];
+#pragma unroll
+            for (int g = 0; g < NG; g++) f[g] = score_factor(c, now.k[g]);
+            w.weigh(s, f);
+#pragma unroll
+            for (int g = 0; g < NG; g++) f[g] = power(now.v[g]);
+            w.add(kt + TB, s, f, lane);
+        } else {
+            w.weigh(s, c);
+            w.add(kt + TB, s, lane);
+        }
     }
     if (__syncthreads_or(odd)) {
         for (int t = all / (KW * kKeys) * (KW * kKeys); t < end; t++)  // (the tiles that were looked through)
@@ -159,22 +180,22 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
             o = o + *reinterpret_cast<const f4*>(sums + (g * QW * 32 + r) * OS + d) * f;
         }
         const int jr = (rho0 + r) / G, h = head * G + (rho0 + r) % G;
-        const float y = len - n + jr + 1 > 0 ? 1.0f / l : 0.f;
+        const float y = limit(jr) > 0 ? 1.0f / l : 0.f;
         *reinterpret_cast<o4*>(static_cast<TO*>(a.out) + (int64_t)(t0 + jr) * a.ldo + (int64_t)h * D + d) =
             o4{(TO)(o[0] * y), (TO)(o[1] * y), (TO)(o[2] * y), (TO)(o[3] * y)};
     }
 }
 
-template <int D, typename T, typename TO>
+template <int D, typename T, typename TO, bool E8>
 struct Prompt {
     template <int QW, int KW>
     static hipError_t launch(const PromptArgs& a, hipStream_t stream) {
-        using S = Shape<D, QW, KW>;
+        using S = Shape<D, QW, KW, E8>;
         const int64_t tiles = tiles_of(a, S::kRows);
         if (tiles * a.cache.kv_heads > UINT32_MAX / S::kThreads) return hipErrorInvalidValue;  // (a launch's threads are counted in 32 bits)
         static std::atomic<uint64_t> devices{0};
-        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW>), S::kLds, devices); e != hipSuccess) return e;
-        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW, E8>), S::kLds, devices); e != hipSuccess) return e;
+        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW, E8>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,
                            a, (int)tiles);
         return hipGetLastError();
     }
@@ -199,7 +220,7 @@ struct Prompt {
 }  // namespace
 
 hipError_t launch_attn_prompt(const PromptArgs& a, int dtype, int out_dtype, hipStream_t stream) {
-    return by_type<Prompt>(a, a.cache.head_dim, dtype, out_dtype, stream);
+    return a.cache.k_scale ? by_type<Prompt, true>(a, a.cache.head_dim, dtype, out_dtype, stream) : by_type<Prompt, false>(a, a.cache.head_dim, dtype, out_dtype, stream);
 }
 
 }  // namespace vxs

@@ -18,7 +18,7 @@
 
 #include <algorithm>
 
-#include "vxs_attn_core.h"
+#include "vxs_attn_core8.h"
 #include "vxs_attn_plan.h"
 #include "vxs_attn_types.h"
 
@@ -29,8 +29,10 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kAtOnce = 8;  // parts that are asked for at once to join them
 
-template <int D>
-constexpr int kTile = D == 64 ? 64 : 32;  // keys of a wave's tile: 8 KiB of keys, 16 at D = 256
+template <int D, bool E8>
+constexpr int kTile = E8 || D == 64 ? 64 : 32;  // keys of a wave's tile: 8 KiB of keys, 16 at D = 256 (8-bit entries: 4 at D = 64)
+template <int D, bool E8>
+constexpr int kRow = E8 ? D : 2 * D;  // bytes of a key
 
 __device__ __forceinline__ void put2(float* p, float a, float b) {
     const uint64_t x = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
@@ -81,18 +83,19 @@ struct KernelArgs {
 
 // LDS of a wave: its tile of keys and its tile of values, later its sums [32][D + 4]; then of the workgroup m and l of each
 // wave's query rows, and what is done after.
-template <int D>
-constexpr int kWaveBytes = 2 * kTile<D> * 2 * D > kCols * (D + 4) * 4 ? 2 * kTile<D> * 2 * D : kCols * (D + 4) * 4;
-template <int D>
-constexpr int kLdsBytes = kWaves * (kWaveBytes<D> + kCols * 8) + kCols * 4;
+template <int D, bool E8>
+constexpr int kWaveBytes = 2 * kTile<D, E8> * kRow<D, E8> > kCols * (D + 4) * 4 ? 2 * kTile<D, E8> * kRow<D, E8> : kCols * (D + 4) * 4;
+template <int D, bool E8>
+constexpr int kLdsBytes = kWaves * (kWaveBytes<D, E8> + kCols * 8) + kCols * 4;
 
-template <int D, typename T, typename TO>
+// T: the queries' type, E8: over 8-bit entries (else of T).
+template <int D, typename T, typename TO, bool E8>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(KernelArgs args) {
-    constexpr int KT = kTile<D>, NB = KT / 32, NG = KT / 16, NI = KT * 2 * D / 1024, TB = KT * 2 * D;
-    constexpr int PARTS = sizeof(TO) == 4 ? Vec<T>::kParts : 1;
+    constexpr int KT = kTile<D, E8>, NB = KT / 32, NG = KT / 16, ROW = kRow<D, E8>, TB = KT * ROW, NI = TB / 1024;
+    constexpr int PARTS = weight_parts<T, TO, E8>;
     constexpr int OS = D + 4;  // floats of a row of the wave's sums
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float* wave_ml = reinterpret_cast<float*>(lds + kWaves * kWaveBytes<D>);  // [waves][32][2]
+    float* wave_ml = reinterpret_cast<float*>(lds + kWaves * kWaveBytes<D, E8>);  // [waves][32][2]
     int* complete = reinterpret_cast<int*>(wave_ml + kWaves * kCols * 2);     // [32]: parts of the rows that are complete
     const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
     const StepArgs& a = args.a;
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     if (!pre) id -= pre_blocks;
     // The threads that share this work: the workgroup's, or the wave's (solo); there are no barriers among the latter.
     const bool solo = !pre && sp.solo;
-    const int tid = solo ? lane : threadIdx.x, threads = solo ? 64 : kThreads, step = solo ? kTile<D> : kWaves * kTile<D>;
+    const int tid = solo ? lane : threadIdx.x, threads = solo ? 64 : kThreads, step = solo ? kTile<D, E8> : kWaves * kTile<D, E8>;
     if (solo) id = id * kWaves + wv;
     auto sync = [&] {
         if (!solo) {
@@ -162,22 +165,27 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     const int32_t* pages = a.cache.table + (int64_t)slot * a.cache.ld_table;
 
     // ---- the wave's tiles begin to load; queries; how many tokens of the slot each sees
-    Loader<D> loader;
+    Loader<D, std::conditional_t<E8, TileGeom8<D>, TileGeom<D>>> loader;
     loader.init(a.cache, lane);
-    char* const kt = lds + wv * kWaveBytes<D>;
+    char* const kt = lds + wv * kWaveBytes<D, E8>;
     char* const vt = kt + TB;
     const unsigned k_lds = lds_address(kt), v_lds = lds_address(vt);
     const char* const k_base = a.cache.k + (uint64_t)head * a.cache.head_stride;
     const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
     const int last_page = (int)a.cache.ld_table - 1;
     uint64_t at[NG];
+    Scales<E8 ? NG : 1> scales;  // of the tile that find() was last asked for
     auto find = [&](int t) {
 #pragma unroll
-        for (int g = 0; g < NG; g++) at[g] = granule_offset(a.cache, pages, last_page, t + 16 * g);
+        for (int g = 0; g < NG; g++) {
+            const int page = granule_page(a.cache, pages, last_page, t + 16 * g);
+            at[g] = cache_offset(a.cache, page, 0, t + 16 * g);
+            if constexpr (E8) scales.read(a.cache, g, page, head, t + 16 * g, c1);
+        }
     };
     auto fetch = [&](const char* base, unsigned to) {
 #pragma unroll
-        for (int g = 0; g < NG; g++) loader.load(base + at[g], to + g * 16 * 2 * D);
+        for (int g = 0; g < NG; g++) loader.load(base + at[g], to + g * 16 * ROW);
     };
     int t = c0 + (solo ? 0 : wv * KT);
     if (t < c1) {
@@ -186,7 +194,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         fetch(v_base, v_lds);
     }
     const int col = lane & 31;
-    Queries<D, T, PARTS> w;
+    std::conditional_t<E8, Queries8<D, T, PARTS>, Queries<D, T, PARTS>> w;
     w.init();
     const int rho = rho0 + min(col, cols - 1);
     const int over = pre ? sp.group.div(rho) : 0, row = rbase + over, qh = head * G + rho - over * G;
@@ -203,20 +211,36 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     bool odd = false;
     for (; t < c1; t += step) {
         const bool more = t + step < c1;
+        const Scales<E8 ? NG : 1> now = scales;
         if (more) find(t + step);
         wait_vm<NI>();
         f16v s[NB];
 #pragma unroll
-        for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 32 * 2 * D, lane);
+        for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 32 * ROW, lane);
         wait_lds();
         if (more) fetch(k_base, k_lds);
         const bool tail = t + KT > c1;
         if (each || tail) w.hide(s, (each ? seen : c1) - t, lane);
-        w.weigh(s, c);
+        if constexpr (E8) {
+            float f[NG];
+#pragma unroll
+            for (int g = 0; g < NG; g++) f[g] = score_factor(c, now.k[g]);
+            w.weigh(s, f);
+        } else {
+            w.weigh(s, c);
+        }
         if (more) wait_vm<NI>();
         else wait_vm<0>();
-        if (each || tail) odd |= scrub<D, T, TB>(vt, t, c1, each, lane);
-        w.add(vt, s, lane);
+        if constexpr (E8) {
+            if (each || tail) odd |= scrub8<D, TB>(vt, t, c1, each, lane);
+            float f[NG];
+#pragma unroll
+            for (int g = 0; g < NG; g++) f[g] = power(now.v[g]);
+            w.add(vt, s, f, lane);
+        } else {
+            if (each || tail) odd |= scrub<D, T, TB>(vt, t, c1, each, lane);
+            w.add(vt, s, lane);
+        }
         wait_lds();
         if (more) fetch(v_base, v_lds);
     }
@@ -254,7 +278,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         for (int i = 0; i < kWaves; i++) {
             const int from = solo ? wv : i;
             x[i] = *reinterpret_cast<const float2*>(wave_ml + (from * kCols + q) * 2);
-            y[i] = *reinterpret_cast<const f4*>(lds + from * kWaveBytes<D> + (q * OS + d) * 4);
+            y[i] = *reinterpret_cast<const f4*>(lds + from * kWaveBytes<D, E8> + (q * OS + d) * 4);
             m = fmaxf(m, x[i].x);
         }
         f4 o{0.f, 0.f, 0.f, 0.f};
@@ -372,7 +396,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     }
 }
 
-template <int D, typename T, typename TO>
+template <int D, typename T, typename TO, bool E8>
 struct Step {
     static hipError_t go(const StepArgs& a, hipStream_t stream) {
         const Split s = plan_step(a, a.work != nullptr);
@@ -381,8 +405,8 @@ struct Step {
         const int64_t blocks = (int64_t)s.pre_tiles * s.pre_parts * a.cache.kv_heads + (s.solo ? (own + kWaves - 1) / kWaves : own);
         if (blocks > UINT32_MAX / kThreads || own > INT32_MAX) return hipErrorInvalidValue;  // (a launch's threads are counted in 32 bits)
         static std::atomic<uint64_t> devices{0};
-        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_step_kernel<D, T, TO>), kLdsBytes<D>, devices); e != hipSuccess) return e;
-        hipLaunchKernelGGL((attn_step_kernel<D, T, TO>), dim3((unsigned)blocks), dim3(kThreads), kLdsBytes<D>, stream, KernelArgs{a, s, r});
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_step_kernel<D, T, TO, E8>), (kLdsBytes<D, E8>), devices); e != hipSuccess) return e;
+        hipLaunchKernelGGL((attn_step_kernel<D, T, TO, E8>), dim3((unsigned)blocks), dim3(kThreads), (kLdsBytes<D, E8>), stream, KernelArgs{a, s, r});
         return hipGetLastError();
     }
 };
@@ -394,7 +418,7 @@ int64_t attn_step_work_bytes(const StepArgs& a) {
 }
 
 hipError_t launch_attn_step(const StepArgs& a, int dtype, int out_dtype, hipStream_t stream) {
-    return by_type<Step>(a, a.cache.head_dim, dtype, out_dtype, stream);
+    return a.cache.k_scale ? by_type<Step, true>(a, a.cache.head_dim, dtype, out_dtype, stream) : by_type<Step, false>(a, a.cache.head_dim, dtype, out_dtype, stream);
 }
 
 }  // namespace vxs

@@ -21,13 +21,13 @@ inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>
     return e;
 }
 
-// F<D, T, TO>::go(a, stream) for head_dim D, the cache's type T and the outputs' type TO.
-template <template <int, typename, typename> class F, typename A>
+// F<D, T, TO, E8>::go(a, stream) for head_dim D, the queries' type T and the outputs' type TO, over entries of T or 8-bit ones.
+template <template <int, typename, typename, bool> class F, bool E8, typename A>
 hipError_t by_type(const A& a, int head_dim, int dtype, int out_dtype, hipStream_t stream) {
     auto dim = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (dtype == VXS_BF16) return out_dtype == VXS_F32 ? F<D, __bf16, float>::go(a, stream) : F<D, __bf16, __bf16>::go(a, stream);
-        return out_dtype == VXS_F32 ? F<D, _Float16, float>::go(a, stream) : F<D, _Float16, _Float16>::go(a, stream);
+        if (dtype == VXS_BF16) return out_dtype == VXS_F32 ? F<D, __bf16, float, E8>::go(a, stream) : F<D, __bf16, __bf16, E8>::go(a, stream);
+        return out_dtype == VXS_F32 ? F<D, _Float16, float, E8>::go(a, stream) : F<D, _Float16, _Float16, E8>::go(a, stream);
     };
     switch (head_dim) {
         case 64: return dim(std::integral_constant<int, 64>{});

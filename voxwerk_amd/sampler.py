@@ -11,13 +11,13 @@ import ctypes
 import os
 import threading
 from dataclasses import dataclass, field
-from typing import Iterable, Optional
+from typing import Iterable, Optional, Union
 
 import numpy as np
 
 from . import _lib
 from ._lib import PARAMS_DTYPE, load_vxs, ptr
-from .attention import DTYPES, KvCache, KvPrep, SharedPrefix
+from .attention import DTYPES, Kv8Cache, KvCache, KvPrep, RopeAxes, SharedPrefix
 
 
 class SamplerError(RuntimeError):
@@ -409,34 +409,50 @@ class Context:
 
     # attention over a paged cache (device pointers, asynchronous; voxwerk_amd.attention has the structures) ----
     def kv_append_device(self, tokens: int, q_heads: int, q, ldq: int, k, ldk: int, v, ldv: int, in_dtype: str,
-                         cache: KvCache, pos, slots, q_out, ld_q_out: int, prep: Optional[KvPrep] = None, index=None,
-                         status=None) -> None:
-        """vxs_kv_append_device: norm and rotate new tokens' query and key heads, queries to q_out, keys and values
-        to their pages."""
-        self._check(self._lib.vxs_kv_append_device(
-            self._h, tokens, q_heads, ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, DTYPES[in_dtype],
-            prep.ref if prep is not None else None, ptr(pos), ptr(slots), ptr(index), cache.ref, ptr(q_out), ld_q_out,
-            ptr(status)))
+                         cache: Union[KvCache, Kv8Cache], pos, slots, q_out, ld_q_out: int, prep: Optional[KvPrep] = None,
+                         index=None, status=None, axes: Optional[RopeAxes] = None) -> None:
+        """vxs_kv_append_device (axes: vxs_kv_append_axes_device; an 8-bit cache: vxs_kv8_append_device): norm and rotate new
+        tokens' query and key heads, queries to q_out, keys and values to their pages."""
+        head = (self._h, tokens, q_heads, ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, DTYPES[in_dtype],
+                prep.ref if prep is not None else None)
+        rest = (ptr(pos), ptr(slots), ptr(index), cache.ref, ptr(q_out), ld_q_out, ptr(status))
+        if cache.bits == 8:
+            self._check(self._lib.vxs_kv8_append_device(*head, axes.ref if axes is not None else None, *rest))
+        elif axes is not None:
+            self._check(self._lib.vxs_kv_append_axes_device(*head, axes.ref, *rest))
+        else:
+            self._check(self._lib.vxs_kv_append_device(*head, *rest))
 
-    def attn_prompt_device(self, seqs: int, tokens: int, q_heads: int, q, ldq: int, cache: KvCache, q_off, kv_len,
+    def attn_prompt_device(self, seqs: int, tokens: int, q_heads: int, q, ldq: int, cache: Union[KvCache, Kv8Cache], q_off, kv_len,
                            scale: float, out, ldo: int, out_dtype: str, slots=None) -> None:
-        """vxs_attn_prompt_device: causal attention of packed sequences' new tokens over their pages."""
-        self._check(self._lib.vxs_attn_prompt_device(self._h, seqs, tokens, q_heads, ptr(q), ldq, cache.ref, ptr(slots),
-                                                     ptr(q_off), ptr(kv_len), scale, ptr(out), ldo, DTYPES[out_dtype]))
+        """vxs_attn_prompt_device, vxs_attn8_prompt_device: causal attention of packed sequences' new tokens over their pages."""
+        call = self._lib.vxs_attn8_prompt_device if cache.bits == 8 else self._lib.vxs_attn_prompt_device
+        self._check(call(self._h, seqs, tokens, q_heads, ptr(q), ldq, cache.ref, ptr(slots), ptr(q_off), ptr(kv_len), scale,
+                         ptr(out), ldo, DTYPES[out_dtype]))
 
-    def attn_step_workspace(self, rows: int, q_heads: int, cache: KvCache, max_len: int,
+    def attn_cross_device(self, seqs: int, tokens: int, q_heads: int, q, ldq: int, cache: Union[KvCache, Kv8Cache], q_off, kv_len,
+                          scale: float, out, ldo: int, out_dtype: str, slots=None) -> None:
+        """vxs_attn_cross_device, vxs_attn8_cross_device: packed tokens over all of their sequences' cached states."""
+        call = self._lib.vxs_attn8_cross_device if cache.bits == 8 else self._lib.vxs_attn_cross_device
+        self._check(call(self._h, seqs, tokens, q_heads, ptr(q), ldq, cache.ref, ptr(slots), ptr(q_off), ptr(kv_len), scale,
+                         ptr(out), ldo, DTYPES[out_dtype]))
+
+    def attn_step_workspace(self, rows: int, q_heads: int, cache: Union[KvCache, Kv8Cache], max_len: int,
                             prefix: Optional[SharedPrefix] = None) -> int:
-        """vxs_attn_step_workspace: the bytes of zeroed device memory that steps of these sizes work in."""
-        n = self._lib.vxs_attn_step_workspace(self._h, rows, q_heads, cache.ref, max_len,
-                                              prefix.ref if prefix is not None else None)
+        """vxs_attn_step_workspace, vxs_attn8_step_workspace: the bytes of zeroed device memory that steps of these sizes work
+        in."""
+        call = self._lib.vxs_attn8_step_workspace if cache.bits == 8 else self._lib.vxs_attn_step_workspace
+        n = call(self._h, rows, q_heads, cache.ref, max_len, prefix.ref if prefix is not None else None)
         self._check(min(n, 0))
         return n
 
-    def attn_step_device(self, rows: int, q_heads: int, q, ldq: int, cache: KvCache, kv_len, max_len: int, scale: float,
-                         out, ldo: int, out_dtype: str, slots=None, prefix: Optional[SharedPrefix] = None,
+    def attn_step_device(self, rows: int, q_heads: int, q, ldq: int, cache: Union[KvCache, Kv8Cache], kv_len, max_len: int,
+                         scale: float, out, ldo: int, out_dtype: str, slots=None, prefix: Optional[SharedPrefix] = None,
                          workspace=None, workspace_bytes: int = 0) -> None:
-        """vxs_attn_step_device: attention of one token per sequence over its pages, shared prefixes read once."""
-        self._check(self._lib.vxs_attn_step_device(
+        """vxs_attn_step_device, vxs_attn8_step_device: attention of one token per sequence over its pages, shared prefixes read
+        once."""
+        call = self._lib.vxs_attn8_step_device if cache.bits == 8 else self._lib.vxs_attn_step_device
+        self._check(call(
             self._h, rows, q_heads, ptr(q), ldq, cache.ref, ptr(slots), ptr(kv_len), max_len,
             prefix.ref if prefix is not None else None, scale, ptr(out), ldo, DTYPES[out_dtype], ptr(workspace),
             workspace_bytes))
