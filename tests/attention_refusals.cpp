@@ -31,7 +31,7 @@ int ctx_ok(vxs_ctx* ctx) {
 }
 hipError_t launch_kv_append(const AppendArgs&, int, int, hipStream_t) { return launches++, hipSuccess; }
 hipError_t launch_kv8_append(const AppendArgs&, int, int, hipStream_t) { return launches++, hipSuccess; }
-hipError_t launch_attn_prompt(const PromptArgs&, int, int, hipStream_t) { return launches++, hipSuccess; }
-hipError_t launch_attn_step(const StepArgs&, int, int, hipStream_t) { return launches++, hipSuccess; }
+hipError_t launch_attn_prompt(const PromptArgs&, const CacheScales&, bool, int, int, hipStream_t) { return launches++, hipSuccess; }
+hipError_t launch_attn_step(const StepArgs&, const CacheScales&, int, int, hipStream_t) { return launches++, hipSuccess; }
 int64_t attn_step_work_bytes(const StepArgs& a) { return work_bytes(a); }
 }  // namespace vxs

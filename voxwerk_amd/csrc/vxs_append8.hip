@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kAT) void kv8_append_kernel(AppendArgs a, int chunk
                     y[i] = load4(src + rb);
                 }
             }
-            uint8_t* const scale = (is_k ? a.cache.k_scale : a.cache.v_scale) + scale_index(a.cache, page, h, block << 4);
+            uint8_t* const scale = (is_k ? a.scales.k : a.scales.v) + scale_index(a.cache, page, h, block << 4);
             const int old = fresh ? 1 : *scale;
 #pragma unroll
             for (int i = 0; i < NI; i++) {

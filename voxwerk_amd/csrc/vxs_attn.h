@@ -12,7 +12,6 @@ namespace vxs {
 struct PagedCache {
     char* k;
     char* v;
-    uint8_t *k_scale, *v_scale;  // of 8-bit entries, else null
     const int32_t* table;
     int64_t ld_table;
     int64_t head_stride;                 // bytes
@@ -20,16 +19,22 @@ struct PagedCache {
     int slots, pages, page_bits, kv_heads, head_dim;
 };
 
+// Scales of 8-bit entries (null: entries of 16 bits).
+struct CacheScales {
+    uint8_t *k, *v;
+};
+
 struct AppendArgs {
     PagedCache cache;
     vxs_kv_prep prep;
-    vxs_rope_axes axes;  // axes 0: one position a token
     const void *q, *k, *v;  // q, or k and v, may be null
     int64_t ldq, ldk, ldv, ldqo;
     const int32_t *pos, *slots, *index;
     void* q_out;
     int32_t* status;
     int tokens, q_heads;
+    vxs_rope_axes axes;  // axes 0: one position a token
+    CacheScales scales;
 };
 hipError_t launch_kv_append(const AppendArgs& a, int in_dtype, int dtype, hipStream_t stream);
 hipError_t launch_kv8_append(const AppendArgs& a, int in_dtype, int q_dtype, hipStream_t stream);
@@ -42,10 +47,10 @@ struct PromptArgs {
     int64_t ldq, ldo;  // elements
     float scale;
     int seqs, tokens, q_heads;
-    int cross;  // every token sees all of its sequence's keys
 };
-// (dtype: the queries' type; 8-bit entries where the cache has scales)
-hipError_t launch_attn_prompt(const PromptArgs& a, int dtype, int out_dtype, hipStream_t stream);
+// dtype: the queries' type; cross: every token sees all of its sequence's keys. The scales come after the other arguments in the kernels:
+// those of 16-bit caches do not move for them (a prompt of 93 tokens took 8.35 us with longer ones, 7.86 with these).
+hipError_t launch_attn_prompt(const PromptArgs& a, const CacheScales& scales, bool cross, int dtype, int out_dtype, hipStream_t stream);
 
 struct StepArgs {
     PagedCache cache;
@@ -60,7 +65,7 @@ struct StepArgs {
 };
 // The bytes of `work` that launch_attn_step asks for at sizes up to a call's (work itself is not looked at).
 int64_t attn_step_work_bytes(const StepArgs& a);
-hipError_t launch_attn_step(const StepArgs& a, int dtype, int out_dtype, hipStream_t stream);
+hipError_t launch_attn_step(const StepArgs& a, const CacheScales& scales, int dtype, int out_dtype, hipStream_t stream);
 
 #ifdef __HIPCC__
 // Tokens that slot `slot` may read: none for a slot outside the cache, at most what its table names.

@@ -24,18 +24,17 @@ constexpr int entry_bytes(const vxs_kv_cache*) { return 2; }
 constexpr int entry_bytes(const vxs_kv8_cache*) { return 1; }
 int query_type(const vxs_kv_cache* c) { return c->dtype; }
 int query_type(const vxs_kv8_cache* c) { return c->q_dtype; }
-int check_scales(vxs_ctx*, const vxs_kv_cache*, vxs::PagedCache&) { return VXS_OK; }
-int check_scales(vxs_ctx* ctx, const vxs_kv8_cache* c, vxs::PagedCache& out) {
+int check_scales(vxs_ctx*, const vxs_kv_cache*, vxs::CacheScales&) { return VXS_OK; }
+int check_scales(vxs_ctx* ctx, const vxs_kv8_cache* c, vxs::CacheScales& out) {
     if (!c->k_scale || !c->v_scale) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "cache k_scale or v_scale is NULL");
     if (((uintptr_t)c->k_scale & 3u) || ((uintptr_t)c->v_scale & 3u))
         return ctx_fail(ctx, VXS_ERR_UNSUPPORTED, "cache needs 4-byte aligned k_scale and v_scale");
-    out.k_scale = c->k_scale;
-    out.v_scale = c->v_scale;
+    out = {c->k_scale, c->v_scale};
     return VXS_OK;
 }
 
 template <typename Cache>
-int check_cache(vxs_ctx* ctx, const Cache* c, int q_heads, vxs::PagedCache& out) {
+int check_cache(vxs_ctx* ctx, const Cache* c, int q_heads, vxs::PagedCache& out, vxs::CacheScales& scales) {
     constexpr int bytes = entry_bytes(static_cast<const Cache*>(nullptr)), unit = 16 / bytes;
     if (!c) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "cache is NULL");
     if (c->slots <= 0 || c->pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->head_dim <= 0 || c->ld_table <= 0)
@@ -62,7 +61,6 @@ int check_cache(vxs_ctx* ctx, const Cache* c, int q_heads, vxs::PagedCache& out)
         return ctx_fail(ctx, VXS_ERR_UNSUPPORTED, "token_stride must stay below 2^25, page_stride below 2^31");
     out.k = static_cast<char*>(c->k);
     out.v = static_cast<char*>(c->v);
-    out.k_scale = out.v_scale = nullptr;
     out.table = c->table;
     out.ld_table = c->ld_table;
     out.page_stride = (uint32_t)(bytes * c->page_stride);
@@ -73,7 +71,7 @@ int check_cache(vxs_ctx* ctx, const Cache* c, int q_heads, vxs::PagedCache& out)
     out.page_bits = __builtin_ctz((unsigned)c->page_size);
     out.kv_heads = c->kv_heads;
     out.head_dim = c->head_dim;
-    return check_scales(ctx, c, out);
+    return check_scales(ctx, c, scales);
 }
 
 template <typename Cache>
@@ -91,8 +89,8 @@ int check_attn(vxs_ctx* ctx, const Cache* c, int q_heads, const void* q, int64_t
 
 template <typename Cache>
 int step_args(vxs_ctx* ctx, int rows, int q_heads, const Cache* cache, int max_len, const vxs_shared_prefix* prefix,
-              vxs::StepArgs& a) {
-    int rc = check_cache(ctx, cache, q_heads, a.cache);
+              vxs::StepArgs& a, vxs::CacheScales& scales) {
+    int rc = check_cache(ctx, cache, q_heads, a.cache, scales);
     if (rc != VXS_OK) return rc;
     if (rows < 0 || max_len < 0) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "bad rows or max_len");
     a.rows = rows;
@@ -115,7 +113,7 @@ int append(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, co
            const int32_t* d_slots, const int32_t* d_index, const Cache* cache, void* q_out, int64_t ldqo, int32_t* d_status) {
     if (!ctx) return VXS_ERR_INVALID_ARG;
     vxs::AppendArgs a{};
-    const int rc = check_cache(ctx, cache, q_heads, a.cache);
+    const int rc = check_cache(ctx, cache, q_heads, a.cache, a.scales);
     if (rc != VXS_OK) return rc;
     if (tokens < 0) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "tokens < 0");
     if (in_dtype != VXS_F32 && in_dtype != VXS_BF16 && in_dtype != VXS_F16)
@@ -166,7 +164,7 @@ int append(vxs_ctx* ctx, int tokens, int q_heads, const void* q, int64_t ldq, co
     a.tokens = tokens;
     a.q_heads = q_heads;
     const auto stream = static_cast<hipStream_t>(vxs_get_stream(ctx));
-    VXS_ATTN_HIP(ctx, a.cache.k_scale ? vxs::launch_kv8_append(a, in_dtype, query_type(cache), stream)
+    VXS_ATTN_HIP(ctx, a.scales.k ? vxs::launch_kv8_append(a, in_dtype, query_type(cache), stream)
                                       : vxs::launch_kv_append(a, in_dtype, query_type(cache), stream));
     return vxs::ctx_ok(ctx);
 }
@@ -177,7 +175,8 @@ int packed(vxs_ctx* ctx, bool cross, int seqs, int tokens, int q_heads, const vo
            int out_dtype) {
     if (!ctx) return VXS_ERR_INVALID_ARG;
     vxs::PromptArgs a{};
-    int rc = check_cache(ctx, cache, q_heads, a.cache);
+    vxs::CacheScales scales{};
+    int rc = check_cache(ctx, cache, q_heads, a.cache, scales);
     if (rc != VXS_OK) return rc;
     if (seqs < 0 || tokens < 0) return ctx_fail(ctx, VXS_ERR_INVALID_ARG, "bad seqs or tokens");
     if ((rc = check_attn(ctx, cache, q_heads, q, ldq, out, ldo, out_dtype, scale)) != VXS_OK) return rc;
@@ -197,8 +196,7 @@ int packed(vxs_ctx* ctx, bool cross, int seqs, int tokens, int q_heads, const vo
     a.seqs = seqs;
     a.tokens = tokens;
     a.q_heads = q_heads;
-    a.cross = cross;
-    VXS_ATTN_HIP(ctx, vxs::launch_attn_prompt(a, query_type(cache), out_dtype, static_cast<hipStream_t>(vxs_get_stream(ctx))));
+    VXS_ATTN_HIP(ctx, vxs::launch_attn_prompt(a, scales, cross, query_type(cache), out_dtype, static_cast<hipStream_t>(vxs_get_stream(ctx))));
     return vxs::ctx_ok(ctx);
 }
 
@@ -208,7 +206,8 @@ int step(vxs_ctx* ctx, int rows, int q_heads, const void* q, int64_t ldq, const 
          int out_dtype, void* work, int64_t work_bytes) {
     if (!ctx) return VXS_ERR_INVALID_ARG;
     vxs::StepArgs a{};
-    int rc = step_args(ctx, rows, q_heads, cache, max_len, prefix, a);
+    vxs::CacheScales scales{};
+    int rc = step_args(ctx, rows, q_heads, cache, max_len, prefix, a, scales);
     if (rc != VXS_OK) return rc;
     if ((rc = check_attn(ctx, cache, q_heads, q, ldq, out, ldo, out_dtype, scale)) != VXS_OK) return rc;
     if (rows == 0) return vxs::ctx_ok(ctx);
@@ -226,7 +225,7 @@ int step(vxs_ctx* ctx, int rows, int q_heads, const void* q, int64_t ldq, const 
     a.ldo = ldo;
     a.scale = scale;
     a.work = work;
-    VXS_ATTN_HIP(ctx, vxs::launch_attn_step(a, query_type(cache), out_dtype, static_cast<hipStream_t>(vxs_get_stream(ctx))));
+    VXS_ATTN_HIP(ctx, vxs::launch_attn_step(a, scales, query_type(cache), out_dtype, static_cast<hipStream_t>(vxs_get_stream(ctx))));
     return vxs::ctx_ok(ctx);
 }
 
@@ -234,7 +233,8 @@ template <typename Cache>
 int64_t workspace(vxs_ctx* ctx, int rows, int q_heads, const Cache* cache, int max_len, const vxs_shared_prefix* prefix) {
     if (!ctx) return VXS_ERR_INVALID_ARG;
     vxs::StepArgs a{};
-    const int rc = step_args(ctx, rows, q_heads, cache, max_len, prefix, a);
+    vxs::CacheScales scales{};
+    const int rc = step_args(ctx, rows, q_heads, cache, max_len, prefix, a, scales);
     return rc != VXS_OK ? rc : vxs::attn_step_work_bytes(a);
 }
 

@@ -52,7 +52,7 @@ __device__ __forceinline__ h8 widen<_Float16>(i2 x, float scale) {
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// The scale's byte of token t's block (uniform), of k_scale or v_scale: scalar loads are of whole words.
+// The scale's byte of token t's block (uniform), of keys or values: scalar loads are of whole words.
 __device__ __forceinline__ unsigned scale_byte(const uint8_t* scales, uint64_t index) {
     return ((unsigned)scalar(reinterpret_cast<const int32_t*>(scales), (int64_t)(index >> 2)) >> (8 * (index & 3))) & 255u;
 }
@@ -60,9 +60,9 @@ __device__ __forceinline__ unsigned scale_byte(const uint8_t* scales, uint64_t i
 template <int N>
 struct Scales {
     unsigned k[N], v[N];
-    __device__ __forceinline__ void read(const PagedCache& c, int g, int page, int head, int t, int end) {
+    __device__ __forceinline__ void read(const PagedCache& c, const CacheScales& scales, int g, int page, int head, int t, int end) {
         const uint64_t at = scale_index(c, page, head, t);
-        const unsigned kb = scale_byte(c.k_scale, at), vb = scale_byte(c.v_scale, at);
+        const unsigned kb = scale_byte(scales.k, at), vb = scale_byte(scales.v, at);
         k[g] = t < end ? kb : 127u;
         v[g] = t < end ? vb : 127u;
     }

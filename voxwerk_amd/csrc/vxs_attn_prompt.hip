@@ -35,9 +35,9 @@ struct Shape {
     static constexpr int kLds = kTiles > kSums ? kTiles : kSums;
 };
 
-// T: the queries' type, E8: over 8-bit entries (else of T).
-template <int D, typename T, typename TO, int QW, int KW, bool E8>
-__global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles) {
+// T: the queries' type, E8: over 8-bit entries (else of T), CROSS: every token sees all of its sequence's keys.
+template <int D, typename T, typename TO, int QW, int KW, bool E8, bool CROSS>
+__global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int tiles, CacheScales entry_scales) {
     using S = Shape<D, QW, KW, E8>;
     constexpr int TB = S::kTile, NB = S::kKeys / 32, NG = S::kKeys / 16, GB = TB / NG, kRows = S::kRows, kKeys = S::kKeys;
     constexpr int PARTS = weight_parts<T, TO, E8>;
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
     const int col = wv * 32 + (lane & 31);
     const int rho = rho0 + min(col, rows - 1);
     const int j = rho / G, qh = head * G + rho % G;
-    auto limit = [&](int j) { return a.cross ? len : max(len - n + j + 1, 0); };  // keys that token j sees
+    auto limit = [&](int j) { return CROSS ? len : max(len - n + j + 1, 0); };  // keys that token j sees
     const int seen = limit(j);
     const int first = uniform(limit((rho0 + min(wv * 32, rows - 1)) / G));  // seen by the wave's first row
     const int last = uniform(limit((rho0 + min(wv * 32 + 31, rows - 1)) / G));
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
         if constexpr (E8)
 #pragma unroll
             for (int g = 0; g < NG; g++)
-                scales.read(a.cache, g, granule_page(a.cache, pages, last_page, t + 16 * g), head, t + 16 * g, end);
+                scales.read(a.cache, entry_scales, g, granule_page(a.cache, pages, last_page, t + 16 * g), head, t + 16 * g, end);
     };
     if (kg * kKeys < end) fetch(kg * kKeys, 0);
     w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
@@ -186,21 +186,33 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
     }
 }
 
+struct Call {
+    PromptArgs a;
+    CacheScales scales;
+    bool cross;
+};
+
 template <int D, typename T, typename TO, bool E8>
 struct Prompt {
     template <int QW, int KW>
-    static hipError_t launch(const PromptArgs& a, hipStream_t stream) {
+    static hipError_t launch(const Call& c, hipStream_t stream) {
+        return c.cross ? launch<QW, KW, true>(c, stream) : launch<QW, KW, false>(c, stream);
+    }
+    template <int QW, int KW, bool CROSS>
+    static hipError_t launch(const Call& c, hipStream_t stream) {
+        const PromptArgs& a = c.a;
         using S = Shape<D, QW, KW, E8>;
         const int64_t tiles = tiles_of(a, S::kRows);
         if (tiles * a.cache.kv_heads > UINT32_MAX / S::kThreads) return hipErrorInvalidValue;  // (a launch's threads are counted in 32 bits)
         static std::atomic<uint64_t> devices{0};
-        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW, E8>), S::kLds, devices); e != hipSuccess) return e;
-        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW, E8>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,
-                           a, (int)tiles);
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_prompt_kernel<D, T, TO, QW, KW, E8, CROSS>), S::kLds, devices); e != hipSuccess) return e;
+        hipLaunchKernelGGL((attn_prompt_kernel<D, T, TO, QW, KW, E8, CROSS>), dim3((unsigned)(tiles * a.cache.kv_heads)), dim3(S::kThreads), S::kLds, stream,
+                           a, (int)tiles, c.scales);
         return hipGetLastError();
     }
     static int64_t tiles_of(const PromptArgs& a, int rows) { return (int64_t)a.tokens * (a.q_heads / a.cache.kv_heads) / rows + a.seqs; }
-    static hipError_t go(const PromptArgs& a, hipStream_t stream) {
+    static hipError_t go(const Call& c, hipStream_t stream) {
+        const PromptArgs& a = c.a;
         // Four groups of two waves (two at D = 256, for the LDS) while 128 rows a workgroup leave compute units idle and a cache
         // may hold more than a few tiles (us, groups / 128 rows: one prompt of 1000 18.8 / 25.5, of 2000, 264 workgroups, 37 / 45,
         // 4 of 500 to 1000, 408 workgroups, 43 / 27; 130 tokens after 8000 91 / 162; one of 93 9.5 / 7.9).
@@ -210,17 +222,18 @@ struct Prompt {
             // late for four (us, eight / four: 4 times 130 after 8000 47 / 56, after 4000 27 / 31, after 2000 18 / 19, one time 64 after
             // 1000 13.0 / 12.5; 16 times 64 after 2000, 576 workgroups, 31 / 26).
             if constexpr (D == 64)
-                if (keys > 2048 && tiles_of(a, 64) * a.cache.kv_heads <= 256) return launch<2, 8>(a, stream);
-            return launch<2, D == 256 ? 2 : 4>(a, stream);
+                if (keys > 2048 && tiles_of(a, 64) * a.cache.kv_heads <= 256) return launch<2, 8>(c, stream);
+            return launch<2, D == 256 ? 2 : 4>(c, stream);
         }
-        return launch<4, 1>(a, stream);
+        return launch<4, 1>(c, stream);
     }
 };
 
 }  // namespace
 
-hipError_t launch_attn_prompt(const PromptArgs& a, int dtype, int out_dtype, hipStream_t stream) {
-    return a.cache.k_scale ? by_type<Prompt, true>(a, a.cache.head_dim, dtype, out_dtype, stream) : by_type<Prompt, false>(a, a.cache.head_dim, dtype, out_dtype, stream);
+hipError_t launch_attn_prompt(const PromptArgs& a, const CacheScales& scales, bool cross, int dtype, int out_dtype, hipStream_t stream) {
+    const Call c{a, scales, cross};
+    return scales.k ? by_type<Prompt, true>(c, a.cache.head_dim, dtype, out_dtype, stream) : by_type<Prompt, false>(c, a.cache.head_dim, dtype, out_dtype, stream);
 }
 
 }  // namespace vxs

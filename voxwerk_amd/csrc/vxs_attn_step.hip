@@ -79,6 +79,7 @@ struct KernelArgs {
     StepArgs a;
     Split sp;
     Records rec;
+    CacheScales scales;
 };
 
 // LDS of a wave: its tile of keys and its tile of values, later its sums [32][D + 4]; then of the workgroup m and l of each
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         for (int g = 0; g < NG; g++) {
             const int page = granule_page(a.cache, pages, last_page, t + 16 * g);
             at[g] = cache_offset(a.cache, page, 0, t + 16 * g);
-            if constexpr (E8) scales.read(a.cache, g, page, head, t + 16 * g, c1);
+            if constexpr (E8) scales.read(a.cache, args.scales, g, page, head, t + 16 * g, c1);
         }
     };
     auto fetch = [&](const char* base, unsigned to) {
@@ -398,7 +399,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
 
 template <int D, typename T, typename TO, bool E8>
 struct Step {
-    static hipError_t go(const StepArgs& a, hipStream_t stream) {
+    static hipError_t go(const KernelArgs& call, hipStream_t stream) {
+        const StepArgs& a = call.a;
         const Split s = plan_step(a, a.work != nullptr);
         const Records r{static_cast<float*>(a.work), s.own_parts + s.pre_parts};
         const int64_t own = (int64_t)a.rows * a.cache.kv_heads * s.head_tiles * s.own_parts;
@@ -406,7 +408,7 @@ struct Step {
         if (blocks > UINT32_MAX / kThreads || own > INT32_MAX) return hipErrorInvalidValue;  // (a launch's threads are counted in 32 bits)
         static std::atomic<uint64_t> devices{0};
         if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(attn_step_kernel<D, T, TO, E8>), (kLdsBytes<D, E8>), devices); e != hipSuccess) return e;
-        hipLaunchKernelGGL((attn_step_kernel<D, T, TO, E8>), dim3((unsigned)blocks), dim3(kThreads), (kLdsBytes<D, E8>), stream, KernelArgs{a, s, r});
+        hipLaunchKernelGGL((attn_step_kernel<D, T, TO, E8>), dim3((unsigned)blocks), dim3(kThreads), (kLdsBytes<D, E8>), stream, KernelArgs{a, s, r, call.scales});
         return hipGetLastError();
     }
 };
@@ -417,8 +419,9 @@ int64_t attn_step_work_bytes(const StepArgs& a) {
     return work_bytes(a);
 }
 
-hipError_t launch_attn_step(const StepArgs& a, int dtype, int out_dtype, hipStream_t stream) {
-    return a.cache.k_scale ? by_type<Step, true>(a, a.cache.head_dim, dtype, out_dtype, stream) : by_type<Step, false>(a, a.cache.head_dim, dtype, out_dtype, stream);
+hipError_t launch_attn_step(const StepArgs& a, const CacheScales& scales, int dtype, int out_dtype, hipStream_t stream) {
+    const KernelArgs call{a, {}, {}, scales};
+    return scales.k ? by_type<Step, true>(call, a.cache.head_dim, dtype, out_dtype, stream) : by_type<Step, false>(call, a.cache.head_dim, dtype, out_dtype, stream);
 }
 
 }  // namespace vxs

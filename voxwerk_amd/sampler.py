@@ -413,15 +413,17 @@ class Context:
                          index=None, status=None, axes: Optional[RopeAxes] = None) -> None:
         """vxs_kv_append_device (axes: vxs_kv_append_axes_device; an 8-bit cache: vxs_kv8_append_device): norm and rotate new
         tokens' query and key heads, queries to q_out, keys and values to their pages."""
-        head = (self._h, tokens, q_heads, ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, DTYPES[in_dtype],
-                prep.ref if prep is not None else None)
-        rest = (ptr(pos), ptr(slots), ptr(index), cache.ref, ptr(q_out), ld_q_out, ptr(status))
-        if cache.bits == 8:
-            self._check(self._lib.vxs_kv8_append_device(*head, axes.ref if axes is not None else None, *rest))
-        elif axes is not None:
-            self._check(self._lib.vxs_kv_append_axes_device(*head, axes.ref, *rest))
-        else:
-            self._check(self._lib.vxs_kv_append_device(*head, *rest))
+        if axes is None and cache.bits == 16:
+            self._check(self._lib.vxs_kv_append_device(
+                self._h, tokens, q_heads, ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, DTYPES[in_dtype],
+                prep.ref if prep is not None else None, ptr(pos), ptr(slots), ptr(index), cache.ref, ptr(q_out), ld_q_out,
+                ptr(status)))
+            return
+        call = self._lib.vxs_kv8_append_device if cache.bits == 8 else self._lib.vxs_kv_append_axes_device
+        self._check(call(
+            self._h, tokens, q_heads, ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, DTYPES[in_dtype],
+            prep.ref if prep is not None else None, axes.ref if axes is not None else None, ptr(pos), ptr(slots), ptr(index),
+            cache.ref, ptr(q_out), ld_q_out, ptr(status)))
 
     def attn_prompt_device(self, seqs: int, tokens: int, q_heads: int, q, ldq: int, cache: Union[KvCache, Kv8Cache], q_off, kv_len,
                            scale: float, out, ldo: int, out_dtype: str, slots=None) -> None:
