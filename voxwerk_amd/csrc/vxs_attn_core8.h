@@ -107,8 +107,59 @@ __device__ __forceinline__ bool scrub8(char* rows, int row0, int end, bool each,
     return found;
 }
 
-// Queries (vxs_attn_core.h) of type T over 8-bit keys and values; weights are bf16, in PARTS.
-template <int D, typename T, int PARTS>
+// A granule of 8-bit keys and values that a wave asks for, and later leaves in LDS in 16 bits, laid out as Loader's tiles: keys of
+// bf16 times their scale, fp16's range may not hold that, so keys of fp16 as they are; values bf16 times their scale.
+template <int D, typename T>
+struct Stager {
+    using G = TileGeom8<D>;
+    u4 k[G::kLoads], v[G::kLoads];
+    unsigned off[G::kLoads];
+    int lane;
+    __device__ __forceinline__ void init(const PagedCache& c, int l) {
+        lane = l;
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++) off[j] = (unsigned)row(j) * (unsigned)c.token_stride + 16u * (unsigned)(lane % G::kUnits);
+    }
+    __device__ __forceinline__ int row(int j) const { return j * G::kRows + lane / G::kUnits; }
+    __device__ __forceinline__ void load(const char* keys, const char* values) {
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++) k[j] = *reinterpret_cast<const u4*>(keys + off[j]);
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++) v[j] = *reinterpret_cast<const u4*>(values + off[j]);
+    }
+    // vxs_attn_core.h's scrub() of the values, the first of which is key `row0`.
+    __device__ __forceinline__ bool scrub(int row0, int end) {
+        unsigned any = 0;
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++) {
+            const bool there = row0 + row(j) < end;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const unsigned odd = odd8(v[j][e]);
+                any |= there ? odd : 0u;
+                v[j][e] = there ? v[j][e] & ~((odd >> 7) * 255u) : 0u;
+            }
+        }
+        return any != 0;
+    }
+    __device__ __forceinline__ void store(char* keys, int values, const Scales<1>& scales) const {
+        constexpr bool kFold = std::is_same_v<T, __bf16>;
+        const float ks = kFold ? power(scales.k[0]) : 1.0f, vs = power(scales.v[0]);
+#pragma unroll
+        for (int j = 0; j < G::kLoads; j++) {
+            const int r = row(j), u = (2 * (lane % G::kUnits)) ^ TileGeom<D>::swizzle(r);
+            char* const p = keys + r * TileGeom<D>::kRow;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                *reinterpret_cast<typename Vec<T>::v8*>(p + ((u ^ i) << 4)) = widen<T>(i2{(int)k[j][2 * i], (int)k[j][2 * i + 1]}, ks);
+                *reinterpret_cast<bf8*>(p + values + ((u ^ i) << 4)) = widen<__bf16>(i2{(int)v[j][2 * i], (int)v[j][2 * i + 1]}, vs);
+            }
+        }
+    }
+};
+
+// Queries (vxs_attn_core.h) of type T over 8-bit keys and values; weights are bf16, in PARTS. STAGED: the tiles are in 16 bits.
+template <int D, typename T, int PARTS, bool STAGED>
 struct Queries8 : Queries<D, __bf16, PARTS> {
     using G = TileGeom8<D>;
     using Base = Queries<D, __bf16, PARTS>;
@@ -119,11 +170,12 @@ struct Queries8 : Queries<D, __bf16, PARTS> {
     v8 q[D / 16];
 
     // row: this lane's query (null: zeros); entries 32 t + 16 (lane / 32) + 0..7 and + 8..15 are the lane's for steps 2 t and 2 t + 1
+    // (staged: the 8 at 16 t + 8 (lane / 32) for step t)
     __device__ __forceinline__ void load(const T* row, int lane) {
 #pragma unroll
         for (int t = 0; t < D / 16; t++) {
             v8 x{};
-            if (row) x = *reinterpret_cast<const v8*>(row + 32 * (t >> 1) + 16 * (lane >> 5) + 8 * (t & 1));
+            if (row) x = *reinterpret_cast<const v8*>(row + (STAGED ? 16 * t + 8 * (lane >> 5) : 32 * (t >> 1) + 16 * (lane >> 5) + 8 * (t & 1)));
             q[t] = x;
         }
     }
@@ -135,9 +187,16 @@ struct Queries8 : Queries<D, __bf16, PARTS> {
     // S^T of 32 keys at `tile`, over their scales
     __device__ __forceinline__ f16v scores(const char* tile, int lane) const {
         const int row = lane & 31;
+        f16v s{};
+        if constexpr (STAGED) {
+            const char* p = tile + row * TileGeom<D>::kRow;
+            const int u = ((lane >> 5) ^ TileGeom<D>::swizzle(row)) << 4;
+#pragma unroll
+            for (int t = 0; t < D / 16; t++) s = Vec<T>::mfma(*reinterpret_cast<const v8*>(p + ((32 * t) ^ u)), q[t], s);
+            return s;
+        }
         const char* p = tile + row * G::kRow;
         const int u = ((lane >> 5) ^ G::swizzle(row)) << 4;
-        f16v s{};
 #pragma unroll
         for (int t = 0; t < D / 32; t++) {
             const u4 x = *reinterpret_cast<const u4*>(p + ((32 * t) ^ u));
@@ -191,6 +250,7 @@ struct Queries8 : Queries<D, __bf16, PARTS> {
         return widen<__bf16>(__builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(p + 16 * t * G::kRow + ((32 * b) ^ (unit << 4)))), scale);
     }
 
+    using Base::add;
     // O^T += V^T P^T over NB x 32 keys; scale: of their values' blocks.
     template <int NB>
     __device__ __forceinline__ void add(const char* tile, const f16v (&s)[NB], const float (&scale)[2 * NB], int lane) {
@@ -206,9 +266,12 @@ struct Queries8 : Queries<D, __bf16, PARTS> {
                 for (int i = PARTS - 1; i >= 0; i--) o[b] = Vec<__bf16>::mfma(v, part[k][i], o[b]);
             }
     }
+};
 
-    // Adds a key's NaN values (row: its values in memory), where this lane's query sees it.
-    __device__ __forceinline__ void add_odd(const char* row, bool sees, int lane) {
+// Adds a key's values that are not finite (row: its values in memory, of 8 bits with E8), where this lane's query sees it.
+template <bool E8, int D, typename T, int PARTS>
+__device__ __forceinline__ void add_odd(Queries<D, T, PARTS>& w, const char* row, bool sees, int lane) {
+    if constexpr (E8) {
         row += 4 * (lane >> 5);
 #pragma unroll
         for (int b = 0; b < D / 32; b++)
@@ -217,9 +280,11 @@ struct Queries8 : Queries<D, __bf16, PARTS> {
                 const unsigned odd = odd8(*reinterpret_cast<const unsigned*>(row + 32 * b + 8 * j));
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if ((odd >> (8 * e)) & 128u && sees) o[b][4 * j + e] = __builtin_nanf("");
+                    if ((odd >> (8 * e)) & 128u && sees) w.o[b][4 * j + e] = __builtin_nanf("");
             }
+    } else {
+        w.add_odd(row, sees, lane);
     }
-};
+}
 
 }  // namespace vxs

@@ -29,10 +29,11 @@ struct Shape {
     static constexpr int kThreads = 64 * QW * KW;
     static constexpr int kRows = 32 * QW;    // query rows of a workgroup
     static constexpr int kKeys = 16 * QW;    // of a tile: each wave loads a granule of 16
-    static constexpr int kTile = kKeys * (E8 ? D : 2 * D);
+    static constexpr int kTile = kKeys * 2 * D;
     static constexpr int kTiles = KW * 4 * kTile;                             // [groups][2 buffers][keys, values]
     static constexpr int kSums = KW == 1 ? 0 : QW * KW * 32 * (D + 4 + 2) * 4;  // [waves][32][D + 4], [waves][32] m and l
-    static constexpr int kLds = kTiles > kSums ? kTiles : kSums;
+    static constexpr int kFactors = KW * 2 * (kKeys / 16) * 4;  // [groups][2 buffers][granules] of 8-bit keys
+    static constexpr int kLds = (kTiles > kSums ? kTiles : kSums) + (E8 ? kFactors : 0);
 };
 
 // T: the queries' type, E8: over 8-bit entries (else of T), CROSS: every token sees all of its sequence's keys.
@@ -66,7 +67,8 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
     const int slot = a.slots ? scalar(a.slots, seq) : seq;
     const int len = (int)cache_length(a.cache, slot, scalar(a.kv_len, seq));
 
-    std::conditional_t<E8, Queries8<D, T, PARTS>, Queries<D, T, PARTS>> w;
+    constexpr bool FACTORS = E8 && !std::is_same_v<T, __bf16>;
+    std::conditional_t<FACTORS, Queries8<D, T, PARTS, true>, Queries<D, T, PARTS>> w;
     w.init();
     const int col = wv * 32 + (lane & 31);
     const int rho = rho0 + min(col, rows - 1);
@@ -79,23 +81,26 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
     const int end = uniform(limit((rho0 + rows - 1) / G));  // that some row sees
     const float c = a.scale * kLog2e;
 
-    Loader<D, std::conditional_t<E8, TileGeom8<D>, TileGeom<D>>> loader;
+    std::conditional_t<E8, Stager<D, T>, Loader<D>> loader;
     loader.init(a.cache, lane);
     const int32_t* pages = a.cache.table + (int64_t)(end ? slot : 0) * a.cache.ld_table;
     const int last_page = (int)a.cache.ld_table - 1;
     const char* const k_base = a.cache.k + (uint64_t)head * a.cache.head_stride;
     const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
     char* const own = lds + kg * 4 * TB;
-    Scales<E8 ? NG : 1> scales;  // of the tile that was last fetched
+    float* const factors = reinterpret_cast<float*>(lds + S::kLds - S::kFactors) + kg * 2 * NG;
+    Scales<1> scales;  // of the granule that was last fetched
     auto fetch = [&](int t, int buffer) {  // each wave 16 of the tile's rows
-        const uint64_t at = granule_offset(a.cache, pages, last_page, t + 16 * wv);
-        const unsigned to = lds_address(own + buffer * 2 * TB + wv * GB);
-        loader.load(k_base + at, to);
-        loader.load(v_base + at, to + TB);
-        if constexpr (E8)
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-                scales.read(a.cache, entry_scales, g, granule_page(a.cache, pages, last_page, t + 16 * g), head, t + 16 * g, end);
+        const int page = granule_page(a.cache, pages, last_page, t + 16 * wv);
+        const uint64_t at = cache_offset(a.cache, page, 0, t + 16 * wv);
+        if constexpr (E8) {
+            loader.load(k_base + at, v_base + at);
+            scales.read(a.cache, entry_scales, 0, page, head, t + 16 * wv, end);
+        } else {
+            const unsigned to = lds_address(own + buffer * 2 * TB + wv * GB);
+            loader.load(k_base + at, to);
+            loader.load(v_base + at, to + TB);
+        }
     };
     if (kg * kKeys < end) fetch(kg * kKeys, 0);
     w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
@@ -104,16 +109,21 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
     int buffer = 0;
     for (int base = 0; base < end; base += KW * kKeys, buffer ^= 1) {
         const int t = base + kg * kKeys;
-        wait_vm<0>();
-        __syncthreads();  // the tiles are there, and nobody reads the other buffers any more
-        const Scales<E8 ? NG : 1> now = scales;
-        if (t + KW * kKeys < end) fetch(t + KW * kKeys, buffer ^ 1);
         char* const kt = own + buffer * 2 * TB;
-        if (base + KW * kKeys > all) {  // some row does not see all of the tiles: each wave looks through its part of the values
+        const bool partly = base + KW * kKeys > all;  // some row does not see all of the tiles: each wave looks through its part of the values
+        if constexpr (E8) {
             if (t < end) {
-                if constexpr (E8) odd |= scrub8<D, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
-                else odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
+                if (partly) odd |= loader.scrub(t + 16 * wv, end);
+                loader.store(kt + wv * GB, TB, scales);
+                if (FACTORS && lane == 0) factors[buffer * NG + wv] = score_factor(c, scales.k[0]);
             }
+        } else {
+            wait_vm<0>();
+        }
+        __syncthreads();  // the tiles are there, and nobody reads the other buffers any more
+        if (t + KW * kKeys < end) fetch(t + KW * kKeys, buffer ^ 1);
+        if (!E8 && partly) {
+            if (t < end) odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
             __syncthreads();
         }
         if (t >= last) continue;
@@ -121,23 +131,20 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
 #pragma unroll
         for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 2 * GB, lane);
         if (t + kKeys > first) w.hide(s, seen - t, lane);
-        if constexpr (E8) {
+        if constexpr (FACTORS) {
             float f[NG];
 #pragma unroll
-            for (int g = 0; g < NG; g++) f[g] = score_factor(c, now.k[g]);
+            for (int g = 0; g < NG; g++) f[g] = factors[buffer * NG + g];
             w.weigh(s, f);
-#pragma unroll
-            for (int g = 0; g < NG; g++) f[g] = power(now.v[g]);
-            w.add(kt + TB, s, f, lane);
         } else {
             w.weigh(s, c);
-            w.add(kt + TB, s, lane);
         }
+        w.add(kt + TB, s, lane);
     }
     if (__syncthreads_or(odd)) {
         for (int t = all / (KW * kKeys) * (KW * kKeys); t < end; t++)  // (the tiles that were looked through)
             if (KW == 1 || t / kKeys % KW == kg)
-                w.add_odd(v_base + granule_offset(a.cache, pages, last_page, t & ~15) + (uint64_t)(t & 15) * a.cache.token_stride, t < seen, lane);
+                add_odd<E8>(w, v_base + granule_offset(a.cache, pages, last_page, t & ~15) + (uint64_t)(t & 15) * a.cache.token_stride, t < seen, lane);
     }
     w.finish_sum();
     using o4 = typename Vec<TO>::v4;

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
         fetch(v_base, v_lds);
     }
     const int col = lane & 31;
-    std::conditional_t<E8, Queries8<D, T, PARTS>, Queries<D, T, PARTS>> w;
+    std::conditional_t<E8, Queries8<D, T, PARTS, false>, Queries<D, T, PARTS>> w;
     w.init();
     const int rho = rho0 + min(col, cols - 1);
     const int over = pre ? sp.group.div(rho) : 0, row = rbase + over, qh = head * G + rho - over * G;
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     const StepArgs& b = again.a;
     if (each && __ballot(odd)) {
         for (t = c0 + wv * KT; t < c1; t += t % KT == KT - 1 ? step - KT + 1 : 1)
-            w.add_odd(b.cache.v + (uint64_t)head * b.cache.head_stride +
+            add_odd<E8>(w, b.cache.v + (uint64_t)head * b.cache.head_stride +
                           granule_offset(b.cache, b.cache.table + (int64_t)slot * b.cache.ld_table, (int)b.cache.ld_table - 1, t & ~15) +
                           (uint64_t)(t & 15) * b.cache.token_stride,
                       t < seen, lane);
