@@ -118,9 +118,10 @@ struct Stager {
     __device__ __forceinline__ void init(const PagedCache& c, int l) {
         lane = l;
 #pragma unroll
-        for (int j = 0; j < G::kLoads; j++) off[j] = (unsigned)row(j) * (unsigned)c.token_stride + 16u * (unsigned)(lane % G::kUnits);
+        for (int j = 0; j < G::kLoads; j++) off[j] = (unsigned)row(j) * (unsigned)c.token_stride + 16u * (unsigned)unit();
     }
     __device__ __forceinline__ int row(int j) const { return j * G::kRows + lane / G::kUnits; }
+    __device__ __forceinline__ int unit() const { return lane % G::kUnits; }
     __device__ __forceinline__ void load(const char* keys, const char* values) {
 #pragma unroll
         for (int j = 0; j < G::kLoads; j++) k[j] = *reinterpret_cast<const u4*>(keys + off[j]);
@@ -147,7 +148,7 @@ struct Stager {
         const float ks = kFold ? power(scales.k[0]) : 1.0f, vs = power(scales.v[0]);
 #pragma unroll
         for (int j = 0; j < G::kLoads; j++) {
-            const int r = row(j), u = (2 * (lane % G::kUnits)) ^ TileGeom<D>::swizzle(r);
+            const int r = row(j), u = (2 * unit()) ^ TileGeom<D>::swizzle(r);
             char* const p = keys + r * TileGeom<D>::kRow;
 #pragma unroll
             for (int i = 0; i < 2; i++) {

@@ -102,34 +102,38 @@ __global__ __launch_bounds__(64 * QW * KW, D == 256 || QW * KW > 8 ? 1 : 2) void
             loader.load(v_base + at, to + TB);
         }
     };
+    bool odd = false;
+    // 8-bit entries: the tile at t, asked for before, goes to its buffer, and the next one is asked for
+    auto stage = [&](int t, int buffer) {
+        if constexpr (E8) {
+            if (t >= end) return;
+            if (t - kg * kKeys + KW * kKeys > all) odd |= loader.scrub(t + 16 * wv, end);
+            loader.store(own + buffer * 2 * TB + wv * GB, TB, scales);
+            if (FACTORS && lane == 0) factors[buffer * NG + wv] = score_factor(c, scales.k[0]);
+            if (t + KW * kKeys < end) fetch(t + KW * kKeys, 0);
+        }
+    };
     if (kg * kKeys < end) fetch(kg * kKeys, 0);
     w.load(col < rows ? static_cast<const T*>(a.q) + (int64_t)(t0 + j) * a.ldq + (int64_t)qh * D : nullptr, lane);
     w.loaded();
-    bool odd = false;
     int buffer = 0;
+    stage(kg * kKeys, 0);
     for (int base = 0; base < end; base += KW * kKeys, buffer ^= 1) {
         const int t = base + kg * kKeys;
         char* const kt = own + buffer * 2 * TB;
         const bool partly = base + KW * kKeys > all;  // some row does not see all of the tiles: each wave looks through its part of the values
-        if constexpr (E8) {
-            if (t < end) {
-                if (partly) odd |= loader.scrub(t + 16 * wv, end);
-                loader.store(kt + wv * GB, TB, scales);
-                if (FACTORS && lane == 0) factors[buffer * NG + wv] = score_factor(c, scales.k[0]);
-            }
-        } else {
-            wait_vm<0>();
-        }
+        if (!E8) wait_vm<0>();
         __syncthreads();  // the tiles are there, and nobody reads the other buffers any more
-        if (t + KW * kKeys < end) fetch(t + KW * kKeys, buffer ^ 1);
+        if (!E8 && t + KW * kKeys < end) fetch(t + KW * kKeys, buffer ^ 1);
         if (!E8 && partly) {
             if (t < end) odd |= scrub<D, T, GB>(kt + TB + wv * GB, t + 16 * wv, end, true, lane);
             __syncthreads();
         }
-        if (t >= last) continue;
+        if (t >= (E8 ? end : last)) continue;  // (8-bit entries: every wave has its part of the next tile to stage)
         f16v s[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 2 * GB, lane);
+        stage(t + KW * kKeys, buffer ^ 1);
         if (t + kKeys > first) w.hide(s, seen - t, lane);
         if constexpr (FACTORS) {
             float f[NG];
