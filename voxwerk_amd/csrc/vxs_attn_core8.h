@@ -67,6 +67,43 @@ struct Scales {
         v[g] = t < end ? vb : 127u;
     }
 };
+// Scales of a tile of N granules on their way through LDS, as its entries: scalar loads would be waited for with the reads of LDS, a round
+// trip to memory for each tile. [2 N] words at `at` are those that hold the bytes, keys' first.
+template <int N>
+struct ScaleWords {
+    unsigned shift[N];  // a granule's byte in its words
+    // One load, older than those of the tile that the caller asks for next. page[g]: of granule t + 16 g (uniform).
+    __device__ __forceinline__ void ask(const PagedCache& c, const CacheScales& scales, const int (&page)[N], int head, int t, unsigned at, int lane) {
+        int mine = page[0];
+#pragma unroll
+        for (int g = 0; g < N; g++) {
+            shift[g] = 8 * ((unsigned)scale_index(c, page[g], head, t + 16 * g) & 3u);
+            if (lane % N == g) mine = page[g];
+        }
+        const uint8_t* const p = ((lane / N) & 1 ? scales.v : scales.k) + (scale_index(c, mine, head, t + 16 * (lane % N)) & ~uint64_t(3));
+        at = uniform((int)at);
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(p) : "m0", "memory");
+#pragma clang diagnostic pop
+    }
+    // The bytes of keys and values, once they are there; granules that begin at `end` or after, which may hold anything, count as 1.
+    __device__ __forceinline__ void read(const char* at, int t, int end, unsigned (&k)[N], unsigned (&v)[N]) const {
+        unsigned w[2 * N];
+#pragma unroll
+        for (int i = 0; i < 2 * N; i += 4) {
+            const u4 x = *reinterpret_cast<const u4*>(at + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[i + e] = x[e];
+        }
+#pragma unroll
+        for (int g = 0; g < N; g++) {
+            const bool there = t + 16 * g < end;
+            k[g] = there ? (w[g] >> shift[g]) & 255u : 127u;
+            v[g] = there ? (w[N + g] >> shift[g]) & 255u : 127u;
+        }
+    }
+};
 __device__ __forceinline__ float power(unsigned byte) { return __uint_as_float(byte << 23); }
 // c 2^(byte - 127) > 0: what a key's product is multiplied by; never zero, which times the -inf of an unseen key would be NaN
 __device__ __forceinline__ float score_factor(float c, unsigned byte) { return fmaxf(__builtin_ldexpf(c, (int)byte - 127), 0x1p-149f); }

@@ -30,7 +30,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kAtOnce = 8;  // parts that are asked for at once to join them
 
 template <int D, bool E8>
-constexpr int kTile = E8 || D == 64 ? 64 : 32;  // keys of a wave's tile: 8 KiB of keys, 16 at D = 256 (8-bit entries: 4 at D = 64)
+constexpr int kTile = D == 64 ? 64 : 32;  // keys of a wave's tile: 8 KiB of keys, 16 at D = 256, half that of 8-bit ones
 template <int D, bool E8>
 constexpr int kRow = E8 ? D : 2 * D;  // bytes of a key
 
@@ -85,7 +85,9 @@ struct KernelArgs {
 // LDS of a wave: its tile of keys and its tile of values, later its sums [32][D + 4]; then of the workgroup m and l of each
 // wave's query rows, and what is done after.
 template <int D, bool E8>
-constexpr int kWaveBytes = 2 * kTile<D, E8> * kRow<D, E8> > kCols * (D + 4) * 4 ? 2 * kTile<D, E8> * kRow<D, E8> : kCols * (D + 4) * 4;
+constexpr int kTileBytes = 2 * kTile<D, E8> * kRow<D, E8> + (E8 ? 256 : 0);  // (and what a load of scales writes)
+template <int D, bool E8>
+constexpr int kWaveBytes = kTileBytes<D, E8> > kCols * (D + 4) * 4 ? kTileBytes<D, E8> : kCols * (D + 4) * 4;
 template <int D, bool E8>
 constexpr int kLdsBytes = kWaves * (kWaveBytes<D, E8> + kCols * 8) + kCols * 4;
 
@@ -175,14 +177,18 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     const char* const v_base = a.cache.v + (uint64_t)head * a.cache.head_stride;
     const int last_page = (int)a.cache.ld_table - 1;
     uint64_t at[NG];
-    Scales<E8 ? NG : 1> scales;  // of the tile that find() was last asked for
+    int page[NG];
+    ScaleWords<NG> scales;
+    char* const scale_words = vt + TB;
     auto find = [&](int t) {
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const int page = granule_page(a.cache, pages, last_page, t + 16 * g);
-            at[g] = cache_offset(a.cache, page, 0, t + 16 * g);
-            if constexpr (E8) scales.read(a.cache, args.scales, g, page, head, t + 16 * g, c1);
+            page[g] = granule_page(a.cache, pages, last_page, t + 16 * g);
+            at[g] = cache_offset(a.cache, page[g], 0, t + 16 * g);
         }
+    };
+    auto fetch_scales = [&](int t) {
+        if constexpr (E8) scales.ask(a.cache, args.scales, page, head, t, lds_address(scale_words), lane);
     };
     auto fetch = [&](const char* base, unsigned to) {
 #pragma unroll
@@ -191,6 +197,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     int t = c0 + (solo ? 0 : wv * KT);
     if (t < c1) {
         find(t);
+        fetch_scales(t);
         fetch(k_base, k_lds);
         fetch(v_base, v_lds);
     }
@@ -212,31 +219,35 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attn_step_kernel(K
     bool odd = false;
     for (; t < c1; t += step) {
         const bool more = t + step < c1;
-        const Scales<E8 ? NG : 1> now = scales;
         if (more) find(t + step);
         wait_vm<NI>();
+        unsigned k_byte[NG], v_byte[NG];
+        if constexpr (E8) scales.read(scale_words, t, c1, k_byte, v_byte);
         f16v s[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) s[b] = w.scores(kt + b * 32 * ROW, lane);
         wait_lds();
-        if (more) fetch(k_base, k_lds);
+        if (more) {
+            fetch_scales(t + step);
+            fetch(k_base, k_lds);
+        }
         const bool tail = t + KT > c1;
         if (each || tail) w.hide(s, (each ? seen : c1) - t, lane);
         if constexpr (E8) {
             float f[NG];
 #pragma unroll
-            for (int g = 0; g < NG; g++) f[g] = score_factor(c, now.k[g]);
+            for (int g = 0; g < NG; g++) f[g] = score_factor(c, k_byte[g]);
             w.weigh(s, f);
         } else {
             w.weigh(s, c);
         }
-        if (more) wait_vm<NI>();
+        if (more) wait_vm<NI + (E8 ? 1 : 0)>();
         else wait_vm<0>();
         if constexpr (E8) {
             if (each || tail) odd |= scrub8<D, TB>(vt, t, c1, each, lane);
             float f[NG];
 #pragma unroll
-            for (int g = 0; g < NG; g++) f[g] = power(now.v[g]);
+            for (int g = 0; g < NG; g++) f[g] = power(v_byte[g]);
             w.add(vt, s, f, lane);
         } else {
             if (each || tail) odd |= scrub<D, T, TB>(vt, t, c1, each, lane);
