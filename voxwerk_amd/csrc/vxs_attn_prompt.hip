@@ -14,6 +14,13 @@
 // 8192^3 reaches 1.39; matrix cores busy half of the time at a clock that their load holds near 1.83 GHz, the rest waits on the
 // exponentials of the same wave. 24 prompts of 500 to 1000, 16 and 8 heads: 100 us with bf16 outputs (head_dim 64: 60, 256: 271), 156 with fp32 ones, which multiply
 // the values three times (fp16 caches twice, with sums apart: 144 to 150). 4 times 65 to 130 tokens after 8000, 32 and 4 heads of 64, fp16: 40 to 42 us, 440 TFLOP/s. One prompt of 93: 8 us.
+//
+// 8-bit entries: each wave asks for a granule of the tile after the next in registers and leaves it in LDS in 16 bits (vxs_attn_core8.h), between
+// the scores of this tile and their weights; conversions at each wave's own reads were as long as the products (prompt of 8192 652 us). With the
+// figures' sizes: 561 to 577 us, 24 prompts with fp32 outputs 158.
+//
+// Cross attention: every token sees all of its slot's keys. 8 times 500 to 1000 tokens over 750 to 1500 8-bit states, 16 heads of 128: 89 us, 590 TFLOP/s;
+// 24 times 4 over as many, 8 key heads of 64, fp16: 15.2 us, 3.6 TB/s, 192 workgroups.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -231,9 +238,10 @@ struct Prompt {
         if (tiles_of(a, 128) * a.cache.kv_heads <= 288 && keys > 256) {
             // D = 64 leaves LDS for eight groups, one workgroup a compute unit: over long contexts, whose tiles arrive too
             // late for four (us, eight / four: 4 times 130 after 8000 47 / 56, after 4000 27 / 31, after 2000 18 / 19, one time 64 after
-            // 1000 13.0 / 12.5; 16 times 64 after 2000, 576 workgroups, 31 / 26).
+            // 1000 13.0 / 12.5; 16 times 64 after 2000, 576 workgroups, 31 / 26; whole states, which nothing hides: 24
+            // times 4 over 750 to 1500 15.2 / 15.8, of 8 bits 18.7 / 21.2).
             if constexpr (D == 64)
-                if (keys > 2048 && tiles_of(a, 64) * a.cache.kv_heads <= 256) return launch<2, 8>(c, stream);
+                if (keys > (c.cross ? 1024 : 2048) && tiles_of(a, 64) * a.cache.kv_heads <= 256) return launch<2, 8>(c, stream);
             return launch<2, D == 256 ? 2 : 4>(c, stream);
         }
         return launch<4, 1>(c, stream);
