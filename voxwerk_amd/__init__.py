@@ -2,7 +2,7 @@
 
 The product is ``lib/libvxs.so`` (C ABI in ``include/vxs_sampler.h``); this package holds its HIP
 sources (``csrc/``), the Python mirror of the reference's sampling surface (``sampler``), the
-paged cache's structures (``attention``), the
+paged caches' structures (``attention``), the
 deterministic synthetic workloads (``workloads``) and the build recipe (``build``).
 """
 from . import _lib  # noqa: F401

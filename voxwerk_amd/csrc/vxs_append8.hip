@@ -253,7 +253,8 @@ hipError_t launch(const AppendArgs& a, hipStream_t stream) {
     // many sequences 11 and 12, 11 and 12; a wave for each item that there might be 150; 97; 11 and 12).
     const int64_t queries = rows * ((qh + kSets * HW - 1) / (kSets * HW));
     const int64_t filled = (2 * kh + queries) / 8, alone = (rows * 2 * ((kh + HW - 1) / HW) + queries + 3) / 4;
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::max(filled, std::min(alone, 2048 / chunks)), 65535));
+    // (a launch's threads are counted in 32 bits)
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({std::max(filled, std::min(alone, 2048 / chunks)), UINT32_MAX / kAT / chunks, 65535}));
     hipLaunchKernelGGL((kv8_append_kernel<D, TI, TO>), dim3((unsigned)chunks, (unsigned)parts), dim3(kAT), 0, stream, a);
     return hipGetLastError();
 }
