@@ -245,7 +245,7 @@ def test_infinite_and_nan(ctx):
 # ---- axes over a 16-bit cache -----------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 300])
+@pytest.mark.parametrize("tokens", [1, 3, 300, 2051])
 @pytest.mark.parametrize("q_heads,kv_heads,dim,rot,interleaved,norm,axes,in_dtype,dtype,page,order", [s for s in SHAPES if s[6] > 1])
 def test_axes_16(ctx, q_heads, kv_heads, dim, rot, interleaved, norm, axes, in_dtype, dtype, page, order, tokens):
     r = np.random.default_rng(dim + tokens)

@@ -7,10 +7,10 @@
 // values to their places in the pages: one pass over the projections' outputs, bound by memory, and by the launch
 // for the few rows of a generation step.
 //
-// Layout: vxs_append.h. A wave takes one token and 512/D heads at a time, so the four angles of a lane are formed once per token.
+// Layout: vxs_append.h. A wave takes one token and 512/D heads at a time, so the four angles of a lane are formed once per token and wave.
 //
 // Measured: 18,000 tokens of 32 + 2 x 8 heads of 128, fp32 to fp16, 122 us: 664 MB at 5.4 TB/s, what a copy reaches; one token of
-// 16 + 2 x 8 heads 3.2 us, 256 of them 4.2 (a launch alone is 2.6).
+// 16 + 2 x 8 heads 3.2 us, 256 of them 4.2 (a launch alone is 2.6); 12,000 tokens of 16 + 2 x 8 bf16 heads with positions of three axes 45.4 us, 4.4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -22,12 +22,14 @@ namespace {
 
 constexpr int kAT = 256;
 
+
 template <int D, typename TI, typename TO>
-__global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a, int waves) {
     constexpr int L = D / 8;    // lanes of a head
     constexpr int HW = 64 / L;  // heads of a wave at a time
-    const int t = blockIdx.x;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x * (kAT / 64 / waves) + wave / waves, first = blockIdx.y * waves + wave % waves;  // `waves` waves of a workgroup take a token
+    if (t >= a.tokens) return;
     const HeadLane<D> at_head(a.prep, lane);
     const int ra = at_head.ra, rb = at_head.rb;
     const int qh = a.q ? a.q_heads : 0, kh = a.k ? a.cache.kv_heads : 0;
@@ -40,9 +42,9 @@ __global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a) {
         const int place = a.index[t], page = place_page(a.cache, a.slots ? a.slots[t] : t, place);
         if (page >= 0) at = (int64_t)cache_offset(a.cache, page, 0, place);
     }
-    if (a.status && threadIdx.x == 0 && blockIdx.y == 0) a.status[t] = kh && at < 0 ? VXS_ERR_ID_OUT_OF_RANGE : 0;
-    const int step = gridDim.y * (kAT / 64) * HW;
-    for (int h0 = (blockIdx.y * (kAT / 64) + (threadIdx.x >> 6)) * HW; h0 < heads; h0 += step) {
+    if (a.status && lane == 0 && first == 0) a.status[t] = kh && at < 0 ? VXS_ERR_ID_OUT_OF_RANGE : 0;
+    const int step = gridDim.y * waves * HW;
+    for (int h0 = first * HW; h0 < heads; h0 += step) {
         const int h = h0 + lane / L;
         if (h >= heads) continue;  // (a whole head's lanes)
         const bool is_q = h < qh, is_k = !is_q && h < qh + kh;
@@ -74,7 +76,10 @@ hipError_t launch(const AppendArgs& a, hipStream_t stream) {
     // A token's heads go to several workgroups until there are 1024 of them.
     const int most = (heads + per_group - 1) / per_group;
     const int parts = std::max(1, std::min({most, (1024 + a.tokens - 1) / a.tokens, 65535}));
-    hipLaunchKernelGGL((kv_append_kernel<D, TI, TO>), dim3(a.tokens, parts), dim3(kAT), 0, stream, a);
+    // Every wave forms the token's angles: two waves a token where its rows are short and tokens many (us, two / four: 12,000 tokens of 16 + 2 x 8 bf16
+    // heads of 128, three axes, 45.4 / 50.4, of 64 21.5 / 25.3, of 256 82 / 85, 2000 8.9 / 8.8; 18,000 of 32 + 2 x 8 fp32 ones 126.7 / 123.2; one: 45.4, 19.4, 87).
+    const int waves = sizeof(TI) == 2 && a.tokens >= 2048 ? 2 : kAT / 64, tokens = kAT / 64 / waves;
+    hipLaunchKernelGGL((kv_append_kernel<D, TI, TO>), dim3((a.tokens + tokens - 1) / tokens, parts), dim3(kAT), 0, stream, a, waves);
     return hipGetLastError();
 }
 
