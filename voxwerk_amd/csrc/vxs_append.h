@@ -8,6 +8,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "vxs_attn.h"
 
 namespace vxs {
@@ -52,19 +54,23 @@ struct HeadLane {
     }
 
     // Cosines and sines of token t's four pairs (1 and 0 where the lane's do not turn).
-    __device__ __forceinline__ void angles(const AppendArgs& a, int t, f4& c, f4& s) const {
+    template <typename Args>
+    __device__ __forceinline__ void angles(const Args& a, int t, f4& c, f4& s) const {
         c = f4{1.f, 1.f, 1.f, 1.f};
         s = f4{0.f, 0.f, 0.f, 0.f};
         if (!turned) return;
         const f4 w = *reinterpret_cast<const f4*>(a.prep.inv_freq + 4 * u);
         int p[4];
-        if (a.axes.axes) {
-            const i4 x = *reinterpret_cast<const i4*>(a.axes.d_axis + 4 * u);
+        bool one = true;
+        if constexpr (std::is_base_of_v<AppendAxesArgs, Args>) {
+            one = a.axes.axes == 0;
+            if (!one) {
+                const i4 x = *reinterpret_cast<const i4*>(a.axes.d_axis + 4 * u);
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = a.pos[min(max(x[e], 0), a.axes.axes - 1) * a.axes.ld_pos + t];
-        } else {
-            p[0] = p[1] = p[2] = p[3] = a.pos[t];
+                for (int e = 0; e < 4; e++) p[e] = a.pos[min(max(x[e], 0), a.axes.axes - 1) * a.axes.ld_pos + t];
+            }
         }
+        if (one) p[0] = p[1] = p[2] = p[3] = a.pos[t];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const double turns = (double)p[e] * ((double)w[e] * 0.15915494309189533577);

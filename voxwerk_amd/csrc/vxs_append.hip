@@ -8,9 +8,11 @@
 // for the few rows of a generation step.
 //
 // Layout: vxs_append.h. A wave takes one token and 512/D heads at a time, so the four angles of a lane are formed once per token and wave.
+// Kernels for one position a token take no axes among their arguments and waves a token as a constant: with both at run time one token took
+// 3.33 us, not 2.96, 256 of them 4.5, not 4.15.
 //
 // Measured: 18,000 tokens of 32 + 2 x 8 heads of 128, fp32 to fp16, 122 us: 664 MB at 5.4 TB/s, what a copy reaches; one token of
-// 16 + 2 x 8 heads 3.2 us, 256 of them 4.2 (a launch alone is 2.6); 12,000 tokens of 16 + 2 x 8 bf16 heads with positions of three axes 45.4 us, 4.4 TB/s.
+// 16 + 2 x 8 heads 3.0 us, 256 of them 4.2 (a launch alone is 2.6); 12,000 tokens of 16 + 2 x 8 bf16 heads with positions of three axes 45.4 us, 4.4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -22,14 +24,15 @@ namespace {
 
 constexpr int kAT = 256;
 
-
-template <int D, typename TI, typename TO>
-__global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a, int waves) {
+// WAVES waves of a workgroup take a token. Args: AppendOneArgs or AppendAxesArgs.
+template <int D, typename TI, typename TO, int WAVES, typename Args>
+__global__ __launch_bounds__(kAT) void kv_append_kernel(Args a) {
     constexpr int L = D / 8;    // lanes of a head
     constexpr int HW = 64 / L;  // heads of a wave at a time
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x * (kAT / 64 / waves) + wave / waves, first = blockIdx.y * waves + wave % waves;  // `waves` waves of a workgroup take a token
-    if (t >= a.tokens) return;
+    constexpr int kTokens = kAT / 64 / WAVES;
+    const int lane = threadIdx.x & 63, wave = kTokens == 1 ? threadIdx.x >> 6 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = kTokens == 1 ? blockIdx.x : blockIdx.x * kTokens + wave / WAVES, first = blockIdx.y * WAVES + wave % WAVES;
+    if (kTokens > 1 && t >= a.tokens) return;
     const HeadLane<D> at_head(a.prep, lane);
     const int ra = at_head.ra, rb = at_head.rb;
     const int qh = a.q ? a.q_heads : 0, kh = a.k ? a.cache.kv_heads : 0;
@@ -43,7 +46,7 @@ __global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a, int waves)
         if (page >= 0) at = (int64_t)cache_offset(a.cache, page, 0, place);
     }
     if (a.status && lane == 0 && first == 0) a.status[t] = kh && at < 0 ? VXS_ERR_ID_OUT_OF_RANGE : 0;
-    const int step = gridDim.y * waves * HW;
+    const int step = gridDim.y * WAVES * HW;
     for (int h0 = first * HW; h0 < heads; h0 += step) {
         const int h = h0 + lane / L;
         if (h >= heads) continue;  // (a whole head's lanes)
@@ -69,6 +72,14 @@ __global__ __launch_bounds__(kAT) void kv_append_kernel(AppendArgs a, int waves)
     }
 }
 
+template <int D, typename TI, typename TO, int WAVES>
+void launch(const AppendArgs& a, int parts, hipStream_t stream) {
+    constexpr int kTokens = kAT / 64 / WAVES;
+    const dim3 grid((a.tokens + kTokens - 1) / kTokens, parts);
+    if (a.axes.axes) hipLaunchKernelGGL((kv_append_kernel<D, TI, TO, WAVES, AppendAxesArgs>), grid, dim3(kAT), 0, stream, a);
+    else hipLaunchKernelGGL((kv_append_kernel<D, TI, TO, WAVES, AppendOneArgs>), grid, dim3(kAT), 0, stream, a);
+}
+
 template <int D, typename TI, typename TO>
 hipError_t launch(const AppendArgs& a, hipStream_t stream) {
     constexpr int per_group = 4 * (512 / D);  // heads of a workgroup at a time
@@ -76,10 +87,15 @@ hipError_t launch(const AppendArgs& a, hipStream_t stream) {
     // A token's heads go to several workgroups until there are 1024 of them.
     const int most = (heads + per_group - 1) / per_group;
     const int parts = std::max(1, std::min({most, (1024 + a.tokens - 1) / a.tokens, 65535}));
-    // Every wave forms the token's angles: two waves a token where its rows are short and tokens many (us, two / four: 12,000 tokens of 16 + 2 x 8 bf16
-    // heads of 128, three axes, 45.4 / 50.4, of 64 21.5 / 25.3, of 256 82 / 85, 2000 8.9 / 8.8; 18,000 of 32 + 2 x 8 fp32 ones 126.7 / 123.2; one: 45.4, 19.4, 87).
-    const int waves = sizeof(TI) == 2 && a.tokens >= 2048 ? 2 : kAT / 64, tokens = kAT / 64 / waves;
-    hipLaunchKernelGGL((kv_append_kernel<D, TI, TO>), dim3((a.tokens + tokens - 1) / tokens, parts), dim3(kAT), 0, stream, a, waves);
+    // Every wave forms its token's angles: two waves a token, not four, where few groups of heads fill them and tokens fill the compute units
+    // (us, two / four, bf16 inputs; 6000 tokens of 16 + 2 x 8 heads of 64, 4 groups, 11.6 / 12.8; of 128, 8 groups, 2048 of them 9.6 / 9.1, 3000
+    // 11.2 / 11.4, 12,000 35.2 / 37.9; 64 + 2 x 8 of 64, 10 groups, 9000 of them 40.3 / 38.5; 64 + 2 x 8 of 128, 20 groups, 6000 48.5 / 44.1;
+    // three axes: 12,000 of 16 + 2 x 8 of 128 39.2 / 46.6; 32 + 2 x 8, 12 groups, 2048 13.0 / 13.0, 6000 25.8 / 26.8; 20 groups 6000 49.5 / 46.6,
+    // 24 groups 12,000 112.7 / 114.3, 24,000 219 / 221).
+    const int groups = (heads + 512 / D - 1) / (512 / D);
+    const bool few = a.axes.axes ? groups <= (a.tokens < 12000 ? 12 : 24) : groups <= 8 && a.tokens >= 400 * groups;
+    if (sizeof(TI) == 2 && a.tokens >= 2048 && few) launch<D, TI, TO, 2>(a, parts, stream);
+    else launch<D, TI, TO, 4>(a, parts, stream);
     return hipGetLastError();
 }
 

@@ -24,7 +24,8 @@ struct CacheScales {
     uint8_t *k, *v;
 };
 
-struct AppendArgs {
+// An append's arguments as far as each kernel needs them: longer ones take longer to launch (vxs_append.hip).
+struct AppendOneArgs {  // one position a token
     PagedCache cache;
     vxs_kv_prep prep;
     const void *q, *k, *v;  // q, or k and v, may be null
@@ -33,7 +34,11 @@ struct AppendArgs {
     void* q_out;
     int32_t* status;
     int tokens, q_heads;
+};
+struct AppendAxesArgs : AppendOneArgs {
     vxs_rope_axes axes;  // axes 0: one position a token
+};
+struct AppendArgs : AppendAxesArgs {
     CacheScales scales;
 };
 hipError_t launch_kv_append(const AppendArgs& a, int in_dtype, int dtype, hipStream_t stream);
