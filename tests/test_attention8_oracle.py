@@ -43,3 +43,9 @@ def test_append_finds_blocks():
     assert got[1, 0][:2] == (120, 120) and got[1, 1][:2] == (128, 128)  # (16 begins a block: its old scale counts for nothing)
     assert got[2, 0][0] == 121 or got[2, 0][:2] == (121, 121)
     assert got[1, 1][2].tolist() == [1] + [-1] * 15
+
+
+def test_append_takes_infinite_entries_for_none():
+    """A block's scale is that of its finite entries: an infinite one beside 7 asks for 7's, which is larger than the old one."""
+    got = o8.append(None, np.full((3, 2), 120), [(2, 3)], np.array([[np.inf, 7.0]]))
+    assert set(got) == {(2, 0)} and got[2, 0][:2] == (121, 121) and got[2, 0][2].tolist() == [-1] * 3 + [0] + [-1] * 12
