@@ -17,14 +17,13 @@
 // heads 7.3 us, one 5.4: slot and place, page, entries, what the block holds, one after the other.
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
-
 #include "vxs_append.h"
+#include "vxs_append_plan.h"
 
 namespace vxs {
 namespace {
 
-constexpr int kAT = 256;
+constexpr int kAT = kAppend8Threads;
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 
@@ -92,12 +91,6 @@ __device__ __forceinline__ void one_row(const AppendArgs& a, const HeadLane<D>& 
     *reinterpret_cast<unsigned*>(row + rb) = to_e4m3(scaled(y, 127 - byte));
     if (lane % HeadLane<D>::kLanes == 0 && (fresh || byte != old)) *scale = (uint8_t)byte;
 }
-
-// A workgroup's waves, and those of the others at its blockIdx.x, share the items of kChunk rows: each block of 16 tokens that
-// begins among them (its rows may go on in the next chunk), a head's keys or values; and each row's queries, kSets wave loads of them.
-constexpr int kSets = 4;
-
-constexpr int kChunk = 16;
 
 template <int D, typename TI, typename TO>
 __global__ __launch_bounds__(kAT, D == 256 ? 3 : 4) void kv8_append_kernel(AppendArgs a) {
@@ -245,17 +238,8 @@ __global__ __launch_bounds__(kAT, D == 256 ? 3 : 4) void kv8_append_kernel(Appen
 
 template <int D, typename TI, typename TO>
 hipError_t launch(const AppendArgs& a, hipStream_t stream) {
-    constexpr int HW = 512 / D;
-    const int kh = a.k ? a.cache.kv_heads : 0, qh = a.q ? a.q_heads : 0;
-    const int64_t chunks = (a.tokens + kChunk - 1) / kChunk, rows = std::min(a.tokens, kChunk);
-    // Two items a wave where rows fill their blocks; where each is alone in its own there are more of them, which get a wave each up to
-    // 2048 workgroups (us, two / one: 24 prompts of 500 to 1000, 32 + 2 x 8 heads, 138 / 146; 16 of 1000 88 / 91; 1100 tokens of one or of as
-    // many sequences 11 and 12, 11 and 12; a wave for each item that there might be 150; 97; 11 and 12).
-    const int64_t queries = rows * ((qh + kSets * HW - 1) / (kSets * HW));
-    const int64_t filled = (2 * kh + queries) / 8, alone = (rows * 2 * ((kh + HW - 1) / HW) + queries + 3) / 4;
-    // (a launch's threads are counted in 32 bits)
-    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({std::max(filled, std::min(alone, 2048 / chunks)), UINT32_MAX / kAT / chunks, 65535}));
-    hipLaunchKernelGGL((kv8_append_kernel<D, TI, TO>), dim3((unsigned)chunks, (unsigned)parts), dim3(kAT), 0, stream, a);
+    const Append8Grid g = plan_append8(a.tokens, a.q ? a.q_heads : 0, a.k ? a.cache.kv_heads : 0, D);
+    hipLaunchKernelGGL((kv8_append_kernel<D, TI, TO>), dim3(g.chunks, g.parts), dim3(kAT), 0, stream, a);
     return hipGetLastError();
 }
 
