@@ -484,7 +484,8 @@ VXS_API int vxs_kv_append_axes_device(vxs_ctx* ctx, int tokens, int q_heads, con
  * scale for each block of 16 tokens and key head, for keys and values apart. Block b of a slot is its tokens 16 b .. 16 b + 15;
  * its scale of head h is the byte (page * kv_heads + h) * (page_size / 16) + (16 b % page_size) / 16 of k_scale, which stands for
  * 2^(byte - 127) (E8M0; 1 to 254), and its entries for e4m3 * 2^(byte - 127). Strides in entries, multiples of 16, k and v
- * 16-byte aligned; k_scale and v_scale 4-byte aligned and read in whole 4-byte words (else VXS_ERR_UNSUPPORTED).
+ * 16-byte aligned, k_scale and v_scale 4-byte aligned (else VXS_ERR_UNSUPPORTED). Scales are read in whole aligned 4-byte words: the
+ * memory of each array is a multiple of four bytes long, up to three more than pages * kv_heads * page_size / 16.
  * q_dtype: the type of queries, VXS_BF16 or VXS_F16.
  */
 typedef struct vxs_kv8_cache {

@@ -42,8 +42,8 @@ class KvCache:
 class Kv8Cache:
     """One layer's cache in 8 bits (vxs_kv8_cache). `k`, `v`: one byte (e4m3) an entry, as [pages, kv_heads, page_size, head_dim]
     or with the given strides in entries; `k_scale`, `v_scale`: bytes (E8M0: b stands for 2^(b - 127)) [pages, kv_heads,
-    page_size / 16], of each 16 tokens; `q_dtype`: the type of queries ("bf16" or "f16"); `table`: int32 [slots, ld_table] page
-    numbers. Takes a KvCache's place in every call."""
+    page_size / 16], of each 16 tokens, in memory of a multiple of four bytes (read in whole words); `q_dtype`: the type of
+    queries ("bf16" or "f16"); `table`: int32 [slots, ld_table] page numbers. Takes a KvCache's place in every call."""
 
     bits = 8
 
