@@ -453,7 +453,10 @@ VXS_API int64_t vxs_attn_step_workspace(vxs_ctx* ctx, int rows, int q_heads, con
 /*
  * Cross attention of packed tokens to another sequence's states (an encoder's): as vxs_attn_prompt_device, but every token
  * [d_q_off[i], d_q_off[i + 1]) sees all d_kv_len[i] tokens of its slot, of which it is none. Both lengths are of any size. One
- * token per sequence, or a few over many states, are a step's rows too: vxs_attn_step_device's see their whole slot.
+ * token per sequence, or a few over many states, are a step's rows too: vxs_attn_step_device's see their whole slot. A few tokens
+ * of few sequences over long states are faster so, with each sequence a group (d_q_off) that shares all its states (d_kv_len),
+ * VXS_FLAG_SHARE_ALWAYS: 4 times 4 tokens over 4000 to 8000 states of head size 128 take 20 us, not 83; 24 times 4 over 1000 to
+ * 2000 of head size 64 take 29, not 19.
  */
 VXS_API int vxs_attn_cross_device(vxs_ctx* ctx, int seqs, int tokens, int q_heads, const void* q, int64_t ldq,
                                   const vxs_kv_cache* cache, const int32_t* d_slots, const int32_t* d_q_off,

@@ -1,5 +1,5 @@
 """GPU checks of packed attention over an 8-bit cache against the 64-bit oracle where a tile's scales are folded in on its way into LDS: blocks whose
-scales are far apart, in each shape of workgroup; and of appends and cross attention at byte offsets past 2^32."""
+scales are far apart, in each shape of workgroup; of cross attention as a step's rows; and of appends and cross attention at byte offsets past 2^32."""
 from __future__ import annotations
 
 import numpy as np
@@ -9,7 +9,8 @@ from oracle import attention8_np as o8
 from voxwerk_amd import hip
 from voxwerk_amd.attention import Kv8Cache, KvPrep, rope_frequencies
 
-from attention_cases import device, out_array, rows_of, run_prompt
+import attention_cases
+from attention_cases import Paged, device, out_array, rows_of, run_prompt, run_step
 from attention8_cases import Paged8, check, run_cross
 
 pytestmark = pytest.mark.gpu
@@ -37,6 +38,24 @@ def test_scales_far_apart(ctx, n, new, dtype, out, dim, cross):
     got = (run_cross if cross else run_prompt)(ctx, paged, q, [0, new], 4, scale, out)
     limits = [n if cross else n - new + j + 1 for j in range(new)]
     check(got, q, limits, lambda i, h: paged.entries(0, limits[i], h), 4, 2, dim, scale, out, "cross" if cross else "prompt")
+
+
+@pytest.mark.parametrize("kind", [Paged, Paged8])
+@pytest.mark.parametrize("dim,dtype,out", [(64, "f16", "f16"), (128, "bf16", "f32"), (256, "bf16", "bf16")])
+def test_few_tokens_over_long_states_as_a_step(ctx, dim, dtype, out, kind):
+    """Rows of a step whose groups share all that their sequence has are a cross call: one to several tokens a sequence, states of any length."""
+    lens, new = [4001, 700, 0, 33, 2050, 31], [4, 1, 3, 2, 9, 5]
+    paged = kind(lens, 2, dim, 16, dtype, seed=dim)
+    off, whose = np.concatenate([[0], np.cumsum(new)]), np.repeat(np.arange(len(new)), new)
+    q = rows_of(len(whose), 8, dim, dtype, paged.rng, scale=2.0)
+    limits = [lens[i] for i in whose]
+    got = run_step(ctx, paged, q, 8, dim**-0.5, out, kv_len=limits, slots=whose, share=list(zip(off[:-1], off[1:], lens)))
+    args = q, limits, lambda r, h: paged.entries(whose[r], limits[r], h), 8, 2, dim, dim**-0.5
+    for y, what in ((got, "step"), (run_cross(ctx, paged, q, off, 8, dim**-0.5, out), "cross")):
+        if kind is Paged8:
+            check(y, *args, out, what)
+        else:
+            attention_cases.check(y, *args, dtype, out, what)
 
 
 def far_pool(paged, far):

@@ -59,7 +59,10 @@ inline Split plan_step(const StepArgs& a, bool work) {
     // Reading a prefix once costs the joining of its parts and a workgroup's wait for the others. It is worth that where reading
     // it for every row takes longer: from about 200 MB of keys and values, much of which comes from the caches (us, shared / not, 8
     // key heads of 128: 16 rows of 2000 15.6 / 14.2, of 8000 20 / 28, 64 of 500 15.6 / 12.5, of 1000 16.3 / 17.3, of 4000 21 / 45,
-    // 128 of 4000 24 / 85; 4 key heads: 64 of 2000 19.1 / 18.7).
+    // 128 of 4000 24 / 85; 4 key heads: 64 of 2000 19.1 / 18.7). 8-bit entries are half as many bytes, but both ways take as long over them (8 bits, 16
+    // bits, rows of 150 to 300 tokens of their own beside: 64 rows of 500 19.9 / 16.5, 21.7 / 19.2, of 1000 21.9 / 22.4, 23.1 / 24.7, of 2000
+    // 23.2 / 33.3, 23.6 / 34.0; 16 of 4000 23.1 / 21.0, 23.4 / 21.1, of 8000 25.1 / 33.4, 25.1 / 30.9; 4 key heads: 64 of 2000 23.5 / 22.8,
+    // 24.1 / 23.0): the rule counts the entries, two bytes each.
     const bool shares = groups > 0 && max_prefix > 0 &&
                         ((a.prefix.flags & VXS_FLAG_SHARE_ALWAYS) || (double)rows * max_prefix * kv_heads * a.cache.head_dim * 4 >= 2e8);
     // Short rows, more than fit at once: a wave each, with nothing to join (us, one wave / four: 1024 of (row, key head) with

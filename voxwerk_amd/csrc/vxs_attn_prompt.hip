@@ -17,10 +17,14 @@
 //
 // 8-bit entries: each wave asks for a granule of the tile after the next in registers and leaves it in LDS in 16 bits (vxs_attn_core8.h), between
 // the scores of this tile and their weights; conversions at each wave's own reads were as long as the products (prompt of 8192 652 us). With the
-// figures' sizes: 561 to 577 us, 24 prompts with fp32 outputs 158.
+// figures' sizes: 561 to 586 us, 24 prompts with fp32 outputs 158 to 161. Queries of fp16, whose scores take a factor for each granule and whose outputs two
+// parts of each weight, need more registers than there are (8 to 324 bytes of scratch a lane, but for most instances of D = 64): the prompt of 8192
+// 901; 24 prompts with 16-bit outputs, fp16 / bf16, 160 / 113, of 64 93 / 67, of 256 568 / 316.
 //
 // Cross attention: every token sees all of its slot's keys. 8 times 500 to 1000 tokens over 750 to 1500 8-bit states, 16 heads of 128: 89 us, 590 TFLOP/s;
-// 24 times 4 over as many, 8 key heads of 64, fp16: 15.2 us, 3.6 TB/s, 192 workgroups.
+// 24 times 4 over as many, 8 key heads of 64, fp16: 15.5 us, 3.6 TB/s, 192 workgroups. A workgroup reads all keys of its 64 or 128 rows: few tokens of few
+// sequences over long states are faster as rows of a step with their sequences as prefix groups (4 times 4 over 4000 to 8000 of 128: 83 us here, 20
+// there; 24 times 4 over 1000 to 2000 of 64: 18.5, 29).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -239,7 +243,9 @@ struct Prompt {
             // D = 64 leaves LDS for eight groups, one workgroup a compute unit: over long contexts, whose tiles arrive too
             // late for four (us, eight / four: 4 times 130 after 8000 47 / 56, after 4000 27 / 31, after 2000 18 / 19, one time 64 after
             // 1000 13.0 / 12.5; 16 times 64 after 2000, 576 workgroups, 31 / 26; whole states, which nothing hides: 24
-            // times 4 over 750 to 1500 15.2 / 15.8, of 8 bits 18.7 / 21.2).
+            // times 4 over 750 to 1500 15.5 / 15.9, of 8 bits 19.3 / 21.6; over 350 to 700 10.8 / 10.3, 11.6 / 12.0; over 500 to 1000 12.6 /
+            // 12.5, 14.5 / 15.7; over 1000 to 2000 18.3 / 18.8, 23.8 / 27.9; 4 times 64 over 550 to 1100 13.0 / 12.3, 16.6 / 16.8; over 100 to
+            // 200 in a table of 2000 7.4 / 6.4, 8.0 / 7.1).
             if constexpr (D == 64)
                 if (keys > (c.cross ? 1024 : 2048) && tiles_of(a, 64) * a.cache.kv_heads <= 256) return launch<2, 8>(c, stream);
             return launch<2, D == 256 ? 2 : 4>(c, stream);
